@@ -345,7 +345,7 @@ def _store8(cache, scales, x, block, off):
 def _plain_append(s):
     case, BS = s["case"], s["case"]["block"]
     seq, place, has = _places(s)
-    at = place.clamp(min=0)
+    at = torch.where(has, place, 0)
     cos, sin = s["cos"][at][:, None], s["sin"][at][:, None]
     q = s["q"].float()
     if s["wq"] is not None:
