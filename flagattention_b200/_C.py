@@ -30,6 +30,8 @@ EXPORTED_SYMBOLS = (
     "fa_flash_bwd_fused", "fa_flash_bwd_fused_stages", "fa_flash_bwd_fused_workspace_bytes", "fa_piecewise_bwd_fused",
     "fa_piecewise_bwd_fused_workspace_bytes",
     "fa_paged_cache_append", "fa_rotary_pair_fwd", "fa_rotary_pair_bwd",
+    "fa_qk_norm_rotary_fwd", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_rotary_cache",
+    "fa_paged_attention_8bit",
     "fa_device_status", "fa_debug_wait_probe", "fa_set_kernel_family", "fa_status_string", "fa_version",
 )
 
@@ -64,6 +66,34 @@ class PagedArgs(ctypes.Structure):
         ("part_out", ctypes.c_void_p), ("part_max", ctypes.c_void_p), ("part_sum", ctypes.c_void_p),
         ("causal_rows", ctypes.c_int32),
     ]
+
+
+class NormRotaryArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "H", "Hk", "L", "D", "rotary_dim", "interleaved",
+                                              "weight_is_f32", "table_rows")] + \
+        [("eps", ctypes.c_float), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+         ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+         ("pos_stride_b", ctypes.c_int64)]
+
+
+class RotaryCacheArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "dtype", "num_tokens", "num_seqs", "num_q_heads", "num_kv_heads", "head_size", "rotary_dim", "interleaved",
+        "block_size", "num_blocks", "table_cols", "block_table_is_i64", "table_rows", "weight_is_f32")] + \
+        [("eps", ctypes.c_float)] + \
+        [f for n in ("query", "key", "value", "out")
+         for f in ((n, ctypes.c_void_p), (n[0] + "_stride_t", ctypes.c_int64), (n[0] + "_stride_h", ctypes.c_int64))] + \
+        [("key_cache", ctypes.c_void_p), ("value_cache", ctypes.c_void_p), ("kv_stride_b", ctypes.c_int64),
+         ("kv_stride_h", ctypes.c_int64), ("kv_stride_t", ctypes.c_int64), ("key_scales", ctypes.c_void_p),
+         ("value_scales", ctypes.c_void_p), ("context_lens", ctypes.c_void_p), ("query_starts", ctypes.c_void_p),
+         ("block_tables", ctypes.c_void_p), ("bt_stride_s", ctypes.c_int64), ("positions", ctypes.c_void_p),
+         ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("q_weight", ctypes.c_void_p),
+         ("k_weight", ctypes.c_void_p)]
+
+
+class Paged8bitArgs(ctypes.Structure):
+    _fields_ = [("paged", PagedArgs), ("key_scales", ctypes.c_void_p), ("value_scales", ctypes.c_void_p),
+                ("num_blocks", ctypes.c_int32), ("table_cols", ctypes.c_int32)]
 
 
 def lib_path():
@@ -144,6 +174,9 @@ def dtype_code(dtype):
 _SHAPE = struct.Struct("@8i2f2Q")                                   # FlashShape
 _TENSOR4 = struct.Struct("@P3q")                                    # Tensor4
 PAGED_ARGS = struct.Struct("@9ifP2q2P3q2PqP2q3Pi4x")                # PagedArgs
+NORM_ROTARY_ARGS = struct.Struct("@10if5Pq")                        # NormRotaryArgs
+ROTARY_CACHE_ARGS = struct.Struct("@14if" + "P2q" * 4 + "2P3q5Pq5P")   # RotaryCacheArgs
+PAGED_8BIT_ARGS = struct.Struct(PAGED_ARGS.format + "2P2i")         # Paged8bitArgs
 _SIGNATURES = {
     "fa_flash_keep_bits_bytes": "p", "fa_flash_fwd_keep": "pppppp" + "plp", "fa_flash_bwd_keep": "p" * 11 + "lplp",
     "fa_flash_fwd": "ppppppp", "fa_flash_fwd_few_rows": "ppppppp", "fa_flash_key_split": "pi", "fa_flash_few_rows_pays": "pi", "fa_flash_bwd": "ppppppppppplp", "fa_flash_bwd_workspace_bytes": "p",
@@ -155,6 +188,8 @@ _SIGNATURES = {
     "fa_rotary_pair_bwd": "iiiiii" + "p" * 6 + "liplpp", "fa_num_splits_heuristic": "iiiiiiii",
     "fa_flash_bwd_fused_workspace_bytes": "p", "fa_flash_bwd_delta_zero": "pppppl" + "p",
     "fa_flash_bwd_fused_stages": "p" * 11 + "lip", "fa_flash_bwd_dkdv": "p" * 10, "fa_flash_bwd_dq": "p" * 9,
+    "fa_qk_norm_rotary_fwd": "pppppp", "fa_qk_norm_rotary_bwd": "p" * 10 + "lp",
+    "fa_qk_norm_rotary_bwd_workspace_bytes": "p", "fa_rotary_cache": "pp", "fa_paged_attention_8bit": "piiiip",
     "fa_piecewise_bwd_dkdv": "pi" + "p" * 12, "fa_piecewise_bwd_dq": "pi" + "p" * 11,
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int32, "l": ctypes.c_int64}

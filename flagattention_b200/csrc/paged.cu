@@ -7,21 +7,9 @@
 // CTA-wide barrier.  The tiny GEMMs (query group padded to 16 rows) run on
 // m16n8k16 tensor-core MMAs so that arithmetic never limits the stream.
 #include "common.cuh"
+#include "paged_parts.cuh"
 
 namespace fa {
-
-// IdxT: the table's entry type, or InPlace where there is no table (FA_BLOCK_TABLE_IN_PLACE)
-struct InPlace {};
-template <typename IdxT>
-__device__ __forceinline__ int64_t phys_block(const void *block_tables, int64_t bt_stride_s,
-                                              int seq, int logical_block) {
-  const int64_t i = (int64_t)seq * bt_stride_s + logical_block;
-  if constexpr (std::is_same<IdxT, InPlace>::value) return i;
-  else return (int64_t) reinterpret_cast<const IdxT *>(block_tables)[i];
-}
-__device__ __forceinline__ int context_len(const fa_paged_args &a, int seq) {
-  return a.context_lens ? a.context_lens[seq] : a.max_context_len;
-}
 
 template <int D>
 struct PagedCfg {
@@ -37,41 +25,6 @@ struct PagedCfg {
   static constexpr int kMergeBytes = kWarps * 16 * D * 4;    // fp32 partial outputs, aliases ring
   static constexpr int kTotal = kRing + (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes);
 };
-
-// How the kernels size the partitions of fa_paged_attention from the lengths themselves; finest == 0: every sequence
-// takes a.partition_size.  Sizes are finest * 2^k.
-struct Sizing {
-  int finest, coarsest;
-  int ctas;    // > 0: the largest size, up to `coarsest`, that leaves the whole call this many CTAs
-  int parts;   // ctas == 0: the smallest size that cuts a sequence into this many at most
-};
-// The lengths of the first 64 sequences, two a lane, requested ahead of their use.
-struct LaneLens {
-  int first, second;
-};
-__device__ __forceinline__ LaneLens lane_lens(const fa_paged_args &a, const Sizing &z) {
-  const int lane = threadIdx.x & 31;
-  return LaneLens{z.ctas > 0 && lane < a.num_seqs ? context_len(a, lane) : 0,
-                  z.ctas > 0 && lane + 32 < a.num_seqs ? context_len(a, lane + 32) : 0};
-}
-// Tokens per partition of a sequence of `ctx` tokens, called by whole warps; never more partitions than the P of the
-// workspace.
-__device__ __forceinline__ int partition_tokens(const fa_paged_args &a, const Sizing &z, LaneLens lens, int ctx, int P) {
-  if (z.finest == 0) return a.partition_size;
-  int k = 0;
-  if (z.ctas > 0) {
-    auto count = [&](int len) { return min(((unsigned)max(len, 0) + z.finest - 1) / z.finest, 1u << 20); };
-    unsigned lane_n = count(lens.first) + count(lens.second);
-    for (int i = (threadIdx.x & 31) + 64; i < a.num_seqs; i += 32) lane_n += count(context_len(a, i));
-    // (a sum below 2^32: at most 2048 sequences)
-    const unsigned long long n = (unsigned long long)__reduce_add_sync(0xffffffffu, lane_n) *
-                                 (a.num_kv_heads * ((a.num_q_heads / a.num_kv_heads + 15) / 16));
-    while ((z.finest << k) < z.coarsest && (n >> (k + 1)) >= (unsigned)z.ctas) ++k;
-  }
-  const int parts = z.ctas > 0 ? P : min(P, z.parts);
-  while ((z.finest << k) < a.partition_size && (long long)parts * (z.finest << k) < ctx) ++k;
-  return z.finest << k;
-}
 
 // HALF: at most 8 query rows, the upper half of the 16-row tile; the lower half serves the remainder of P.
 template <typename T, int D, typename IdxT, bool HALF>
@@ -539,7 +492,7 @@ static int decode(const fa_paged_args *a, const Sizing &z, cudaStream_t s) {
                                : dispatch_paged_d<__nv_bfloat16, int32_t>(a, z, s);
 }
 
-static int reduce(const fa_paged_args *a, const Sizing &z, cudaStream_t s) {
+int reduce(const fa_paged_args *a, const Sizing &z, cudaStream_t s) {
   dim3 grid(a->num_seqs, a->num_q_heads);
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -552,11 +505,6 @@ static int reduce(const fa_paged_args *a, const Sizing &z, cudaStream_t s) {
   if (st != cudaSuccess) return FA_ERR_LAUNCH;
   FA_CHECK_LAUNCH();
   return FA_OK;
-}
-
-// size / finest is a power of two
-static bool nests(int size, int finest) {
-  return size % finest == 0 && ((size / finest) & (size / finest - 1)) == 0;
 }
 
 }  // namespace fa
@@ -577,11 +525,8 @@ extern "C" int fa_paged_reduce(const fa_paged_args *a, void *stream) {
 extern "C" int fa_paged_attention(const fa_paged_args *a, int32_t finest, int32_t coarsest, int32_t ctas,
                                   int32_t parts, void *stream) {
   if (int st = validate_paged(a, true)) return st;
-  if (a->partition_size <= 0 || a->partition_size > (1 << 24) || finest <= 0 || finest % 16 || finest > a->partition_size ||
-      coarsest < finest || coarsest > (1 << 24) || !nests(a->partition_size, finest) || !nests(coarsest, finest))
-    return FA_ERR_BAD_ARG;
-  if (ctas < 0 || (ctas == 0 && parts <= 0) || (ctas > 0 && a->num_seqs > 2048)) return FA_ERR_BAD_ARG;
   const Sizing z{finest, coarsest, ctas, parts};
+  if (!sizing_ok(*a, z)) return FA_ERR_BAD_ARG;
   if (int st = decode(a, z, static_cast<cudaStream_t>(stream))) return st;
   return reduce(a, z, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,565 @@
+// paged_attention_8bit decode: paged.cu's gather over a cache of e4m3 codes with an fp32 scale for each block and kv head.
+//
+// HBM-bound as there: every warp streams 32-token groups of codes and their scales through a cp.async ring of its own.
+// Codes go to fp16 (exactly) on the way from shared memory to the tensor cores, and two things follow from bytes:
+//  * S = Q K^T contracts over the head, in whatever order both operands agree on: a lane takes 16 codes that lie side by
+//    side as four steps of its K fragment, so K needs neither ldmatrix nor a transposition, and Q's fragments are read
+//    in that order.
+//  * O = P V contracts over tokens, whose codes lie apart: a lane reads the same 16 head elements of four tokens and
+//    interleaves them two by two (one byte permutation for two conversions). Columns of the accumulator are head
+//    elements in that order, so a lane ends with consecutive ones.
+// Which 8 tokens a fragment's columns mean (token_of) and where a row's 16-byte pieces lie (code_offset) are chosen so that
+// both reads hit every bank once.
+//
+// The scale of K goes into the score.  The scale of V cannot go into the accumulator, which many blocks share, nor into
+// P alone, whose 16 bits would not hold its range: a token's weight in O is exp2(score) 2^E f for a scale 2^E f, 1 <= f < 2,
+// and O has a running reference of its own over score + E, beside the maximum that the sum of the softmax goes by.  So
+// weights stay in range whatever the scales are (0 too: E = -inf).
+// bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): elements down to 2^-38 of
+// the maximum keep their bits or lose less than 2^-40 of it.
+#include "common.cuh"
+#include "paged_parts.cuh"
+
+namespace fa {
+
+// Weights of O run up to 2^(kLift + 8 + 1) and so stay in fp16; the lift keeps 2^kLift more of the small ones above its
+// least number.
+constexpr float kLift = 6.f;
+
+template <int D>
+struct Paged8Cfg {
+  static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
+  static constexpr int kWarps = D <= 128 ? 4 : 2;
+  static constexpr int kStages = D <= 64 ? 4 : 3;
+  static constexpr int kTokens = 32;                          // tokens of a group
+  static constexpr int kGroupBytes = kTokens * kD;            // of K or of V
+  static constexpr int kStageBytes = 2 * kGroupBytes;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kQBytes = 16 * kD * 2;
+  static constexpr int kScales = kQBytes;                     // per warp and stage: K, V of the first 16 tokens, K, V of the others
+  static constexpr int kRowScale = kScales + kWarps * kStages * 16;
+  static constexpr int kStats = kRowScale + 16 * 4;           // per warp and row: maximum, sum, reference of O
+  static constexpr int kRing = (kStats + 3 * kWarps * 16 * 4 + 127) / 128 * 128;
+  static constexpr int kRingBytes = kWarps * kWarpBytes;
+  static constexpr int kMergeBytes = kWarps * 16 * kD * 4;    // fp32 partial outputs, over the ring
+  static constexpr int kTotal = kRing + (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes);
+};
+
+// the token, of 8, that column n of a score fragment stands for
+template <int KD>
+__device__ __forceinline__ constexpr int token_of(int n) {
+  const int n0 = n & 1, n1 = n >> 1 & 1, n2 = n >> 2;
+  return KD == 64 ? n2 << 2 | n1 << 1 | (n0 ^ n2) : (n0 ^ n2) << 2 | n1 << 1 | n0;
+}
+// byte offset of 16-byte piece `piece` of row `row` in a group
+template <int KD>
+__device__ __forceinline__ constexpr uint32_t code_offset(int row, int piece) {
+  return (uint32_t)(row * KD + 16 * (KD == 64 ? piece ^ (row & 2) : piece ^ (row & 7)));
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+// two e4m3 codes of a word, as two fp16 numbers
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  uint32_t h;
+  asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}\n" : "=r"(h) : "r"(w));
+  return h;
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  uint32_t h;
+  asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, hi;}\n" : "=r"(h) : "r"(w));
+  return h;
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src));
+}
+// scale = 2^exponent x fraction, 1 <= fraction < 2; 0 (and what is below the normal numbers) has exponent -inf, an
+// infinity or NaN is its own fraction
+__device__ __forceinline__ void split_scale(float scale, float &exponent, float &fraction) {
+  const uint32_t bits = __float_as_uint(scale), e = bits >> 23 & 255u;
+  exponent = e == 255u ? 0.f : e ? (float)((int)e - 127) : -INFINITY;
+  fraction = e == 255u ? scale : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+}
+
+// HALF: at most 8 query rows, the upper half of the 16-row tile; the lower half serves the remainder of P.
+template <typename T, int D, typename IdxT, bool HALF>
+__global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
+    paged_8bit_kernel(const __grid_constant__ fa_paged_8bit_args p, const Sizing z) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the reduction waits for all of this grid by itself
+  using C = Paged8Cfg<D>;
+  constexpr int KD = C::kD, NW = C::kWarps, NS = C::kStages, GT = C::kTokens;
+  constexpr int R = HALF ? 1 : 2;   // accumulator rows of a thread: g and, in a full tile, g + 8
+  constexpr int KJ = KD / 64;       // 16-byte pieces of a row that a lane of a quad takes for S
+  constexpr int VW = KD / 32;       // 4-byte words of a row that a lane takes for O
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  const uint32_t smem = smem_u32(smem_raw);
+  const fa_paged_args &a = p.paged;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int seq = blockIdx.x;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int q_tiles = (G + 15) / 16;
+  const int hk = blockIdx.y / q_tiles, qt = blockIdx.y % q_tiles;
+  const int part = blockIdx.z;
+  const int rows = min(16, G - qt * 16);          // valid query rows of this CTA
+  const int qh0 = hk * G + qt * 16;               // first query head
+
+  const int ctx = context_len(a, seq);
+  int t_begin = 0, t_end = ctx;
+  if (a.partition_size > 0) {
+    const LaneLens lens = lane_lens(a, z);   // in flight together with ctx
+    if ((long long)part * (z.finest ? z.finest : a.partition_size) >= ctx) return;
+    const int size = partition_tokens(a, z, lens, ctx, gridDim.z);
+    if ((long long)part * size >= ctx) return;
+    t_begin = part * size;
+    t_end = (int)min((long long)ctx, (long long)t_begin + size);
+  }
+  const int BS = a.block_size;
+  t_end = (int)min((long long)t_end, (long long)p.table_cols * BS);   // (a table narrower than the length)
+
+  // ---- this warp's token groups ---------------------------------------------
+  const int n_groups = t_end > t_begin ? (t_end - t_begin + GT - 1) / GT : 0;
+  const int my_groups = n_groups > warp ? (n_groups - warp + NW - 1) / NW : 0;
+  const uint32_t ring = smem + C::kRing + warp * C::kWarpBytes;
+  const uint32_t scales = smem + C::kScales + warp * NS * 16;
+  const uint8_t *kc = static_cast<const uint8_t *>(a.key_cache) + (int64_t)hk * a.kv_stride_h;
+  const uint8_t *vc = static_cast<const uint8_t *>(a.value_cache) + (int64_t)hk * a.kv_stride_h;
+  const int64_t v_minus_k = vc - kc;
+  const int bs_shift = (BS & (BS - 1)) == 0 ? 31 - __clz(BS) : -1;
+
+  // A lane copies 16-byte piece `ch` of rows c * RPC + lane_r of a group, of K and of V.
+  constexpr int CPR = D / 16, RPC = 32 / CPR, NC = GT / RPC;
+  const int lane_r = lane / CPR, ch = lane % CPR;
+  uint32_t dst_off[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) dst_off[c] = code_offset<KD>(c * RPC + lane_r, ch);
+  const int64_t lane_src = (int64_t)lane_r * a.kv_stride_t + ch * 16;
+
+  // blocks of the two halves of this warp's i-th group, looked up a group ahead of their use; -1 where the half holds no
+  // token of the partition, -2 for an id outside the cache
+  int64_t next[2];
+  auto look_up = [&](int i) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int tok = t_begin + (warp + i * NW) * GT + 16 * s;
+      next[s] = -1;
+      if (i < my_groups && tok < t_end) {
+        const int64_t id = phys_block<IdxT>(a.block_tables, a.bt_stride_s, seq, bs_shift >= 0 ? tok >> bs_shift : tok / BS);
+        next[s] = id >= 0 && id < p.num_blocks ? id : -2;
+      }
+    }
+  };
+  auto issue = [&](int i) {   // i-th group of this warp -> stage i % NS
+    const int tok0 = t_begin + (warp + i * NW) * GT;
+    const uint32_t st = ring + (i % NS) * C::kStageBytes;
+    const int64_t blk[2] = {next[0], next[1]};
+    look_up(i + 1);
+    const uint8_t *src[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int tok = tok0 + 16 * s;
+      const int in_blk = bs_shift >= 0 ? tok & (BS - 1) : tok % BS;
+      // (the s-th half's rows are counted from the group's start)
+      src[s] = kc + max(blk[s], (int64_t)0) * a.kv_stride_b + (int64_t)(in_blk - 16 * s) * a.kv_stride_t + lane_src;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int row = c * RPC + lane_r, s = row / 16;
+      const bool ok = tok0 + row < t_end && (s ? blk[1] : blk[0]) >= 0;
+      const uint8_t *sk = ok ? (s ? src[1] : src[0]) + (int64_t)(c * RPC) * a.kv_stride_t : kc;
+      cp_async16(st + dst_off[c], sk, ok);
+      cp_async16(st + C::kGroupBytes + dst_off[c], sk + v_minus_k, ok);
+    }
+    if (lane < 4) {
+      const uint32_t at = scales + (i % NS) * 16 + lane * 4;
+      const int64_t id = lane < 2 ? blk[0] : blk[1];
+      const float *from = lane & 1 ? p.value_scales : p.key_scales;
+      if (id >= 0) cp_async4(at, from + id * a.num_kv_heads + hk);
+      // a block outside the cache makes its sequence's output NaN; a half without tokens counts as nothing
+      else asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(at), "f"(id == -2 ? NAN : 0.f) : "memory");
+    }
+  };
+
+  look_up(0);
+  if (D < KD) {   // the padding of shorter heads
+    for (int i = tid; i < C::kRingBytes / 16; i += NW * 32)
+      reinterpret_cast<uint4 *>(smem_raw + C::kRing)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    if (i < my_groups) issue(i);
+    cp_async_commit();
+  }
+
+  // ---- query group -> shared as fp16 (rows >= `rows` are zero) -----------------
+  float *row_scale = reinterpret_cast<float *>(smem_raw + C::kRowScale);
+  {
+    constexpr int TPR = NW * 32 / 16, PIECES = KD / 8 / TPR;   // threads of a row, and their 8-element pieces
+    const int r = tid / TPR, t = tid % TPR;
+    const T *q = static_cast<const T *>(a.query) + (int64_t)seq * a.q_stride_s + (int64_t)(qh0 + r) * a.q_stride_h;
+    uint4 u[PIECES];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int piece = t + i * TPR;
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows && piece * 8 < D) u[i] = *reinterpret_cast<const uint4 *>(q + piece * 8);
+      if (!std::is_same<T, __half>::value) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = Elem<T>::unpack(w[k]);
+          most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+    }
+    float up = 1.f, down = 1.f;
+    if (!std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int m = 1; m < TPR; m *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+      if (most > 0.f && most < INFINITY) {
+        // 2^(14 - exponent of the maximum), inside the normal numbers, and its inverse
+        const int e = min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -126), 126);
+        up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      if (!std::is_same<T, __half>::value) {
+        uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = Elem<T>::unpack(w[k]);
+          w[k] = Elem<__half>::pack(f.x * up, f.y * up);
+        }
+        u[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      *reinterpret_cast<uint4 *>(smem_raw + (r * KD + (t + i * TPR) * 8) * 2) = u[i];
+    }
+    if (t == 0) row_scale[r] = a.attn_scale * kLog2e * down;
+  }
+  __syncthreads();
+
+  float q_scale[2];
+#pragma unroll
+  for (int r = 0; r < R; ++r) q_scale[r] = row_scale[g + 8 * r];
+  // step (j, w) of the contraction is elements 64 j + 16 t4 + 4 w .. + 3 of a row
+  constexpr bool kQInRegs = D <= 128;
+  auto q_step = [&](int j, int w, uint32_t (&qa)[4]) {
+    const uint32_t at = smem + (uint32_t)(g * KD + 64 * j + 16 * t4 + 4 * w) * 2;
+    const uint2 x = lds8(at), y = HALF ? make_uint2(0, 0) : lds8(at + 8 * KD * 2);
+    qa[0] = x.x, qa[1] = y.x, qa[2] = x.y, qa[3] = y.y;
+  };
+  uint32_t qf[kQInRegs ? 4 * KJ : 1][4];
+  if (kQInRegs) {
+#pragma unroll
+    for (int i = 0; i < 4 * KJ; ++i) q_step(i / 4, i % 4, qf[i]);
+  }
+
+  float acc[KD / 8][4];
+#pragma unroll
+  for (int j = 0; j < KD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  float m_i[2] = {-INFINITY, -INFINITY};   // running maximum of the scores
+  float w_i[2] = {-INFINITY, -INFINITY};   // and of score + exponent of V's scale, the reference of acc
+  float l_i[2] = {0.f, 0.f};
+
+#pragma unroll 1
+  for (int i = 0; i < my_groups; ++i) {
+    if (i + NS - 1 < my_groups) issue(i + NS - 1);
+    cp_async_commit();
+    cp_async_wait<NS - 1>();
+    __syncwarp();
+
+    const int tok0 = t_begin + (warp + i * NW) * GT;
+    const uint32_t st = ring + (i % NS) * C::kStageBytes, sv = st + C::kGroupBytes;
+    const uint4 sc = lds16(scales + (i % NS) * 16);
+    const float ks[2] = {__uint_as_float(sc.x), __uint_as_float(sc.z)};
+    float ve[2], vf[2];
+    split_scale(__uint_as_float(sc.y), ve[0], vf[0]);
+    split_scale(__uint_as_float(sc.w), ve[1], vf[1]);
+
+    float s[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+      uint4 k[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) k[n] = lds16(st + code_offset<KD>(8 * n + token_of<KD>(g), 4 * j + t4));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t qa[4];
+        if (!kQInRegs) q_step(j, w, qa);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t kw = w == 0 ? k[n].x : w == 1 ? k[n].y : w == 2 ? k[n].z : k[n].w;
+          Elem<__half>::mma(s[n], kQInRegs ? qf[4 * j + w] : qa, codes_lo(kw), codes_hi(kw));
+        }
+      }
+    }
+    const bool tail = tok0 + GT > t_end;
+    const int col[2] = {token_of<KD>(2 * t4), token_of<KD>(2 * t4 + 1)};
+    float m_new[2], w_new[2];
+    bool need = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx[2] = {-INFINITY, -INFINITY};   // of either half: they have scales of their own
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float &x = s[n][2 * r + e];
+          x = tail && tok0 + 8 * n + col[e] >= t_end ? -INFINITY : x * (q_scale[r] * ks[n >> 1]);
+          mx[n >> 1] = fmaxf(mx[n >> 1], x);
+        }
+      m_new[r] = fmaxf(m_i[r], quad_max(fmaxf(mx[0], mx[1])));
+      w_new[r] = fmaxf(w_i[r], quad_max(fmaxf(mx[0] + ve[0], mx[1] + ve[1])));
+      // lazy, as in paged.cu: a reference moves when it is 2^8 behind
+      need = need || m_new[r] - m_i[r] > 8.f || w_new[r] - w_i[r] > 8.f;
+    }
+    if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        l_i[r] *= m_new[r] == -INFINITY ? 1.f : fast_exp2(m_i[r] - m_new[r]);
+        const float alpha = w_new[r] == -INFINITY ? 1.f : fast_exp2(w_i[r] - w_new[r]);
+        m_i[r] = m_new[r], w_i[r] = w_new[r];
+#pragma unroll
+        for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4 / R; ++e) acc[j][2 * r + e] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float m_ref = m_i[r] == -INFINITY ? 0.f : m_i[r];   // all scores -inf: P = 0
+      const float w_ref = w_i[r] == -INFINITY ? 0.f : w_i[r] - kLift;
+      const float shift[2] = {ve[0] - w_ref, ve[1] - w_ref};
+      float rs = 0.f;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float &x = s[n][2 * r + e];
+          rs += fast_exp2(x - m_ref);
+          x = fast_exp2(x + shift[n >> 1]) * vf[n >> 1];
+        }
+      l_i[r] += rs;
+    }
+    // P goes in as a 16-bit value and a 16-bit remainder, as in paged.cu
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // 16 tokens each
+      uint32_t pa[4], pr[4];
+      if (HALF) {
+        split_weights<__half>(s[2 * h][0], s[2 * h][1], pa[0], pa[1]);
+        split_weights<__half>(s[2 * h + 1][0], s[2 * h + 1][1], pa[2], pa[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          split_weights<__half>(s[2 * h + (k >> 1)][2 * (k & 1)], s[2 * h + (k >> 1)][2 * (k & 1) + 1], pa[k], pr[k]);
+      }
+#pragma unroll
+      for (int j = 0; j < (VW + 3) / 4; ++j) {
+        constexpr int W = VW < 4 ? VW : 4;
+        uint32_t v[4][W];   // tokens 2 t4, 2 t4 + 1 of the first eight and of the second
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 16 * h + 8 * (k >> 1) + col[k & 1];
+          if constexpr (W == 4) {
+            const uint4 x = lds16(sv + code_offset<KD>(row, g + 8 * j));
+            v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+          } else {
+            const uint2 x = lds8(sv + code_offset<KD>(row, g >> 1) + 8 * (g & 1));
+            v[k][0] = x.x, v[k][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t x0 = __byte_perm(v[0][w], v[1][w], 0x5140), x1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+          const uint32_t y0 = __byte_perm(v[2][w], v[3][w], 0x5140), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+          const uint32_t b0[4] = {codes_lo(x0), codes_hi(x0), codes_lo(x1), codes_hi(x1)};
+          const uint32_t b1[4] = {codes_lo(y0), codes_hi(y0), codes_lo(y1), codes_hi(y1)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) Elem<__half>::mma(acc[16 * j + 4 * w + e], pa, b0[e], b1[e]);
+          if (!HALF) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Elem<__half>::mma(acc[16 * j + 4 * w + e], pr, b0[e], b1[e]);
+          }
+        }
+      }
+    }
+    __syncwarp();  // stage may be refilled by the next iteration's issue
+  }
+  cp_async_wait<0>();
+
+  if (HALF) {
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
+  }
+
+  // ---- merge the warps' partial states --------------------------------------
+  float *stat_m = reinterpret_cast<float *>(smem_raw + C::kStats);
+  float *stat_l = stat_m + NW * 16, *stat_w = stat_l + NW * 16;
+  float *merge = reinterpret_cast<float *>(smem_raw + C::kRing);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float l = quad_sum(l_i[r]);
+    if (t4 == 0) {
+      stat_m[warp * 16 + g + 8 * r] = m_i[r];
+      stat_l[warp * 16 + g + 8 * r] = l;
+      stat_w[warp * 16 + g + 8 * r] = w_i[r];
+    }
+  }
+  __syncthreads();  // stats visible; every warp has drained its ring
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = g + 8 * r;
+    if (row >= rows) continue;
+    float ww = -INFINITY;
+#pragma unroll
+    for (int w2 = 0; w2 < NW; ++w2) ww = fmaxf(ww, stat_w[w2 * 16 + row]);
+    const float scale_w = w_i[r] == -INFINITY ? 0.f : fast_exp2(w_i[r] - ww);
+    // a thread's columns 2 t4 and 2 t4 + 1 of the accumulators are two runs of VW words' elements
+    constexpr int W = VW < 4 ? VW : 4;
+#pragma unroll
+    for (int j = 0; j < (VW + 3) / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float(&x)[4] = acc[16 * j + 4 * w], (&y)[4] = acc[16 * j + 4 * w + 1];
+          const float(&u)[4] = acc[16 * j + 4 * w + 2], (&v)[4] = acc[16 * j + 4 * w + 3];
+          const int k = 2 * r + e;
+          *reinterpret_cast<float4 *>(merge + (warp * 16 + row) * KD + 128 * j + 4 * W * (2 * t4 + e) + 4 * w) =
+              make_float4(x[k] * scale_w, y[k] * scale_w, u[k] * scale_w, v[k] * scale_w);
+        }
+  }
+  __syncthreads();
+
+  for (int idx = tid; idx < rows * (D / 4); idx += NW * 32) {
+    const int row = idx / (D / 4), c4 = idx % (D / 4);
+    float mm = -INFINITY, ww = -INFINITY;
+#pragma unroll
+    for (int w2 = 0; w2 < NW; ++w2) {
+      mm = fmaxf(mm, stat_m[w2 * 16 + row]);
+      ww = fmaxf(ww, stat_w[w2 * 16 + row]);
+    }
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w2 = 0; w2 < NW; ++w2) {
+      const float mw = stat_m[w2 * 16 + row];
+      if (mw != -INFINITY) l += stat_l[w2 * 16 + row] * fast_exp2(mw - mm);
+      else l += stat_l[w2 * 16 + row];   // 0, or NaN where every score was
+      const float4 v = *reinterpret_cast<const float4 *>(merge + (w2 * 16 + row) * KD + c4 * 4);
+      o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    }
+    // from the reference of O to that of the sum; a sequence without tokens has 0, a NaN stays one
+    const float inv = l == 0.f ? 0.f : (ww == -INFINITY ? 1.f : fast_exp2(ww - kLift - mm)) / l;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    const int qh = qh0 + row;
+    if (a.partition_size > 0) {
+      const int P = (a.max_context_len + a.partition_size - 1) / a.partition_size;
+      const int64_t pi = ((int64_t)seq * a.num_q_heads + qh) * P + part;
+      *reinterpret_cast<float4 *>(a.part_out + pi * D + c4 * 4) = o;
+      if (c4 == 0) {
+        a.part_max[pi] = mm;
+        a.part_sum[pi] = l;
+      }
+    } else {
+      T *dst = reinterpret_cast<T *>(a.out) + (int64_t)seq * a.o_stride_s +
+               (int64_t)qh * a.o_stride_h + c4 * 4;
+      uint2 pk;
+      pk.x = Elem<T>::pack(o.x, o.y);
+      pk.y = Elem<T>::pack(o.z, o.w);
+      *reinterpret_cast<uint2 *>(dst) = pk;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static int validate_8bit(const fa_paged_8bit_args *p) {
+  if (!p) return FA_ERR_BAD_ARG;
+  const fa_paged_args *a = &p->paged;
+  if (!a->query || !a->key_cache || !a->value_cache || !a->out || !a->context_lens || !a->block_tables ||
+      !p->key_scales || !p->value_scales)
+    return FA_ERR_BAD_ARG;
+  if (a->dtype != FA_F16 && a->dtype != FA_BF16) return FA_ERR_BAD_ARG;
+  if (a->num_seqs <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->block_size <= 0 ||
+      a->max_context_len <= 0 || a->partition_size < 0 || p->num_blocks < 0 || p->table_cols < 0)
+    return FA_ERR_BAD_ARG;
+  if (a->num_q_heads % a->num_kv_heads != 0 || a->block_size % 16 != 0 || a->partition_size % 16 != 0 ||
+      a->causal_rows != 0 || (a->block_table_is_i64 != 0 && a->block_table_is_i64 != 1))
+    return FA_ERR_BAD_ARG;
+  const int D = a->head_size;
+  if (!(D == 16 || D == 32 || D == 64 || D == 128 || D == 256)) return FA_ERR_UNSUPPORTED;
+  if (!aligned16(a->query) || !aligned16(a->key_cache) || !aligned16(a->value_cache) || !aligned16(a->out))
+    return FA_ERR_ALIGNMENT;
+  if (a->q_stride_s % 8 || a->q_stride_h % 8 || a->kv_stride_b % 16 || a->kv_stride_h % 16 ||
+      a->kv_stride_t % 16 || a->o_stride_s % 4 || a->o_stride_h % 4)
+    return FA_ERR_ALIGNMENT;
+  if (a->partition_size > 0 && (!a->part_out || !a->part_max || !a->part_sum)) return FA_ERR_WORKSPACE;
+  const int64_t q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;   // (what a grid holds)
+  if (a->num_kv_heads * q_tiles > 65535 || a->num_q_heads > 65535 ||
+      (a->partition_size > 0 && (a->max_context_len - 1) / a->partition_size >= 65535))
+    return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+template <typename T, int D, typename IdxT, bool HALF>
+static int launch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_t stream) {
+  using C = Paged8Cfg<D>;
+  const fa_paged_args *a = &p->paged;
+  auto kern = paged_8bit_kernel<T, D, IdxT, HALF>;
+  static unsigned long long attr_done = 0;  // per instantiation, one bit per device
+  if (int st = ensure_dyn_smem(kern, C::kTotal, &attr_done)) return st;
+  const int q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;
+  const int P = a->partition_size > 0 ? (a->max_context_len + a->partition_size - 1) / a->partition_size : 1;
+  kern<<<dim3(a->num_seqs, a->num_kv_heads * q_tiles, P), C::kWarps * 32, C::kTotal, stream>>>(*p, z);
+  FA_CHECK_LAUNCH();
+  return FA_OK;
+}
+
+template <typename T, typename IdxT>
+static int dispatch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_t s) {
+  const bool half = p->paged.num_q_heads / p->paged.num_kv_heads <= 8;
+  switch (p->paged.head_size) {
+    case 16: return half ? launch_8bit<T, 16, IdxT, true>(p, z, s) : launch_8bit<T, 16, IdxT, false>(p, z, s);
+    case 32: return half ? launch_8bit<T, 32, IdxT, true>(p, z, s) : launch_8bit<T, 32, IdxT, false>(p, z, s);
+    case 64: return half ? launch_8bit<T, 64, IdxT, true>(p, z, s) : launch_8bit<T, 64, IdxT, false>(p, z, s);
+    case 128: return half ? launch_8bit<T, 128, IdxT, true>(p, z, s) : launch_8bit<T, 128, IdxT, false>(p, z, s);
+    default: return half ? launch_8bit<T, 256, IdxT, true>(p, z, s) : launch_8bit<T, 256, IdxT, false>(p, z, s);
+  }
+}
+
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" int fa_paged_attention_8bit(const fa_paged_8bit_args *p, int32_t finest, int32_t coarsest, int32_t ctas,
+                                       int32_t parts, void *stream) {
+  if (int st = validate_8bit(p)) return st;
+  const fa_paged_args *a = &p->paged;
+  const Sizing z{finest, coarsest, ctas, parts};
+  if (finest && !sizing_ok(*a, z)) return FA_ERR_BAD_ARG;
+  auto s = static_cast<cudaStream_t>(stream);
+  int st;
+  if (a->dtype == FA_F16)
+    st = a->block_table_is_i64 ? dispatch_8bit<__half, int64_t>(p, z, s) : dispatch_8bit<__half, int32_t>(p, z, s);
+  else
+    st = a->block_table_is_i64 ? dispatch_8bit<__nv_bfloat16, int64_t>(p, z, s)
+                               : dispatch_8bit<__nv_bfloat16, int32_t>(p, z, s);
+  if (st != FA_OK || a->partition_size == 0) return st;
+  return reduce(a, z, s);
+}

@@ -1,0 +1,450 @@
+// RMS norm of every head of q and k and their rotation by position, in one pass:
+//   n = x r w,  r = 1 / sqrt(mean(x^2) + eps);   y = R(p) n on the first `rotary_dim` elements, y = n on the others,
+// and its backward:
+//   h = R(p)^T g;  dw = sum over rows of h x r;  a = h w;  dx = r (a - x r mean(a x r)).
+// All of it is fp32 from 16-bit operands, each result rounded once.  HBM-bound: 4 bytes of traffic an element forward, 6
+// backward, some ten operations.
+//
+// A row's 16 D / 16 elements go to the LPR = 2^k >= D / 16 lanes of a group (rotary_pair's layout: 8 rotation pairs a
+// thread in either pair layout, or 16 elements that only pass), so the row's sum is a few shuffles.  A group keeps the
+// cos / sin values of its position and the weights in registers and walks heads of that position, the loads of
+// `kAhead` heads in flight; q and k share the launch (a small call is bound by launches), a CTA has heads of one of them.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "attn_params.cuh"
+#include "common.cuh"
+#include "flagattn_b200.h"
+#include "rotary_common.cuh"
+
+namespace fa {
+
+constexpr int kNormThreads = 128;
+constexpr int kAhead = 4;      // heads whose loads are in flight, forward
+constexpr int kAheadBwd = 2;   // backward: two tensors a head, and the sums of dw in registers
+
+struct NormSide {   // q or k
+  const void *x, *g;
+  void *y;          // forward: the result; backward: dx
+  Strides sx, sg, sy;
+  const void *weight;
+  int heads;
+};
+struct NormArgs {
+  NormSide side[2];
+  const float *cos, *sin;
+  const int64_t *positions;
+  int64_t pos_stride_b;
+  float eps;
+  int B, L, D, R, table_rows, weight_is_f32;
+  int per_cta[2];   // heads a CTA walks
+  int chunks[2];    // and the CTAs that share a position's heads
+  int tiles;        // backward: groups of positions a CTA walks
+};
+
+__device__ __forceinline__ uint4 load16(const void *p) { return *reinterpret_cast<const uint4 *>(p); }
+
+template <typename T>
+__device__ __forceinline__ void load_weight8(float (&w)[8], const void *weight, int at, bool f32) {
+  if (f32) load8(w, static_cast<const float *>(weight) + at);
+  else unpack8<T>(w, load16(static_cast<const T *>(weight) + at));
+}
+
+// What a thread of a group holds for all its heads.
+template <typename T, int LPR, bool IL>
+struct NormLane {
+  int off_a, off_b, b, l, h_lo, h_hi, e;   // e: 0 q, 1 k
+  bool live;
+  float c[8], s[8], wlo[8], whi[8];
+
+  __device__ __forceinline__ void place(const NormArgs &a) {
+    const int j = threadIdx.x % LPR;
+    const bool turns = j < a.R / 16;
+    off_a = IL || !turns ? 16 * j : 8 * j;
+    off_b = IL || !turns ? 16 * j + 8 : a.R / 2 + 8 * j;
+    live = j < a.D / 16;
+    const int Z = a.chunks[0] + a.chunks[1];
+    int z = blockIdx.x % Z;
+    e = z >= a.chunks[0];
+    if (e) z -= a.chunks[0];
+    h_lo = z * a.per_cta[e];
+    h_hi = min(a.side[e].heads, h_lo + a.per_cta[e]);
+    b = (blockIdx.x / Z) % a.B;
+  }
+  __device__ __forceinline__ void weights(const NormArgs &a) {
+    float wa[8], wb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wa[i] = wb[i] = 1.f;
+    const void *w = a.side[e].weight;
+    if (live && w) {
+      load_weight8<T>(wa, w, off_a, a.weight_is_f32);
+      load_weight8<T>(wb, w, off_b, a.weight_is_f32);
+    }
+    to_pairs<IL>(wlo, whi, wa, wb);
+  }
+  // the position of row `row` of the batch element, and its angles
+  __device__ __forceinline__ void turn_to(const NormArgs &a, int row) {
+    l = row;
+    const int j = threadIdx.x % LPR;
+    const bool here = live && l < a.L;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+    if (here && j < a.R / 16) {
+      int64_t pos = a.positions ? a.positions[b * a.pos_stride_b + l] : l;
+      // a position outside the tables reads the nearest row instead of foreign memory
+      pos = pos < 0 ? 0 : (pos >= a.table_rows ? a.table_rows - 1 : pos);
+      const int64_t at = pos * (a.R / 2) + 8 * j;
+      load8(c, a.cos + at);
+      load8(s, a.sin + at);
+    }
+  }
+};
+
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < LPR; m *= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+template <typename T, int LPR, bool IL>
+__global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_fwd_kernel(const NormArgs a) {
+  NormLane<T, LPR, IL> t;
+  t.place(a);
+  const int rows = kNormThreads / LPR;
+  const int Z = a.chunks[0] + a.chunks[1];
+  t.turn_to(a, (int)(blockIdx.x / ((unsigned)Z * a.B)) * rows + threadIdx.x / LPR);
+  t.weights(a);
+  const bool here = t.live && t.l < a.L;
+  const NormSide &side = a.side[t.e];
+  const T *x = static_cast<const T *>(side.x) + t.b * side.sx.b + (here ? t.l * side.sx.l : 0);
+  T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0);
+  const float inv_d = 1.f / a.D;
+
+  for (int h0 = t.h_lo; h0 < t.h_hi; h0 += kAhead) {
+    uint4 ua[kAhead], ub[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
+      if (here && h0 + u < t.h_hi) {
+        const T *src = x + (int64_t)(h0 + u) * side.sx.h;
+        ua[u] = load16(src + t.off_a);
+        ub[u] = load16(src + t.off_b);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (h0 + u >= t.h_hi) break;   // the same for the whole CTA
+      float va[8], vb[8], lo[8], hi[8], ylo[8], yhi[8];
+      unpack8<T>(va, ua[u]);
+      unpack8<T>(vb, ub[u]);
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(va[i], va[i], fmaf(vb[i], vb[i], ss));
+      const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, a.eps));
+      to_pairs<IL>(lo, hi, va, vb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float nl = lo[i] * r * t.wlo[i], nh = hi[i] * r * t.whi[i];
+        ylo[i] = nl * t.c[i] - nh * t.s[i];
+        yhi[i] = nh * t.c[i] + nl * t.s[i];
+      }
+      from_pairs<IL>(va, vb, ylo, yhi);
+      if (here) {
+        T *dst = y + (int64_t)(h0 + u) * side.sy.h;
+        *reinterpret_cast<uint4 *>(dst + t.off_a) = pack8<T>(va);
+        *reinterpret_cast<uint4 *>(dst + t.off_b) = pack8<T>(vb);
+      }
+    }
+  }
+}
+
+// The rows of dw's partial sums, one a CTA of q or of k: partial[0 .. n_q) and [n_q .. n_q + n_k) of D floats, in an order
+// that depends on the shape alone, as do the sums: dw is the same bits every time.
+template <typename T, int LPR, bool IL>
+__global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_bwd_kernel(const NormArgs a, float *partial) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the sum of the partial rows waits for all of this grid
+  constexpr int kRows = kNormThreads / LPR, kWarps = kNormThreads / 32;
+  __shared__ float sums[kWarps][16 * LPR];
+  NormLane<T, LPR, IL> t;
+  t.place(a);
+  t.weights(a);
+  const int Z = a.chunks[0] + a.chunks[1];
+  const int first = (int)(blockIdx.x / ((unsigned)Z * a.B));
+  const NormSide &side = a.side[t.e];
+  const float inv_d = 1.f / a.D;
+  float dlo[8], dhi[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dlo[i] = dhi[i] = 0.f;
+
+  for (int tile = 0; tile < a.tiles; ++tile) {
+    const int row0 = (first * a.tiles + tile) * kRows;
+    if (row0 >= a.L) break;
+    t.turn_to(a, row0 + threadIdx.x / LPR);
+    const bool here = t.live && t.l < a.L;
+    const T *x = static_cast<const T *>(side.x) + t.b * side.sx.b + (here ? t.l * side.sx.l : 0);
+    const T *g = static_cast<const T *>(side.g) + t.b * side.sg.b + (here ? t.l * side.sg.l : 0);
+    T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0);
+    for (int h0 = t.h_lo; h0 < t.h_hi; h0 += kAheadBwd) {
+      uint4 ua[kAheadBwd], ub[kAheadBwd], ga[kAheadBwd], gb[kAheadBwd];
+#pragma unroll
+      for (int u = 0; u < kAheadBwd; ++u) {
+        ua[u] = ub[u] = ga[u] = gb[u] = make_uint4(0, 0, 0, 0);
+        if (here && h0 + u < t.h_hi) {
+          const T *sx = x + (int64_t)(h0 + u) * side.sx.h, *sg = g + (int64_t)(h0 + u) * side.sg.h;
+          ua[u] = load16(sx + t.off_a);
+          ub[u] = load16(sx + t.off_b);
+          ga[u] = load16(sg + t.off_a);
+          gb[u] = load16(sg + t.off_b);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAheadBwd; ++u) {
+        if (h0 + u >= t.h_hi) break;
+        float va[8], vb[8], xlo[8], xhi[8], glo[8], ghi[8];
+        unpack8<T>(va, ua[u]);
+        unpack8<T>(vb, ub[u]);
+        to_pairs<IL>(xlo, xhi, va, vb);
+        unpack8<T>(va, ga[u]);
+        unpack8<T>(vb, gb[u]);
+        to_pairs<IL>(glo, ghi, va, vb);
+        float ss = 0.f, ax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = fmaf(xlo[i], xlo[i], fmaf(xhi[i], xhi[i], ss));
+          const float hl = glo[i] * t.c[i] + ghi[i] * t.s[i], hh = ghi[i] * t.c[i] - glo[i] * t.s[i];
+          glo[i] = hl, ghi[i] = hh;
+          ax = fmaf(hl * t.wlo[i], xlo[i], fmaf(hh * t.whi[i], xhi[i], ax));
+        }
+        const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, a.eps));
+        const float k = group_sum<LPR>(ax) * inv_d * r * r;   // dx = r (a - k x)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dlo[i] = fmaf(glo[i], xlo[i] * r, dlo[i]);
+          dhi[i] = fmaf(ghi[i], xhi[i] * r, dhi[i]);
+          glo[i] = r * (glo[i] * t.wlo[i] - k * xlo[i]);
+          ghi[i] = r * (ghi[i] * t.whi[i] - k * xhi[i]);
+        }
+        from_pairs<IL>(va, vb, glo, ghi);
+        if (here) {
+          T *dst = y + (int64_t)(h0 + u) * side.sy.h;
+          *reinterpret_cast<uint4 *>(dst + t.off_a) = pack8<T>(va);
+          *reinterpret_cast<uint4 *>(dst + t.off_b) = pack8<T>(vb);
+        }
+      }
+    }
+  }
+
+  if (!partial) return;
+  // groups of a warp, then warps, then one row
+  float va[8], vb[8];
+  from_pairs<IL>(va, vb, dlo, dhi);
+#pragma unroll
+  for (int m = LPR; m < 32; m *= 2)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      va[i] += __shfl_xor_sync(0xffffffffu, va[i], m);
+      vb[i] += __shfl_xor_sync(0xffffffffu, vb[i], m);
+    }
+  if ((threadIdx.x & 31) < LPR && t.live) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sums[threadIdx.x / 32][t.off_a + i] = va[i];
+      sums[threadIdx.x / 32][t.off_b + i] = vb[i];
+    }
+  }
+  __syncthreads();
+  // this CTA's row among those of its side: CTAs of a side in order
+  const int z = (int)(blockIdx.x % Z) - (t.e ? a.chunks[0] : 0);
+  const int64_t rest = blockIdx.x / Z, sides = gridDim.x / Z;
+  const int64_t row = (t.e ? sides * a.chunks[0] : 0) + rest * a.chunks[t.e] + z;
+  for (int d = threadIdx.x; d < a.D; d += kNormThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v += sums[w][d];
+    partial[row * a.D + d] = v;
+  }
+}
+
+// dw from the partial rows: a CTA has 8 columns of one side, 128 threads a column, and adds them in a fixed order.
+struct WeightGrad {
+  void *out[2];
+  int rows[2];
+};
+template <typename T>
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float *partial, WeightGrad w, int D, int f32) {
+  __shared__ float sums[128][9];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int e = blockIdx.y, col = blockIdx.x * 8 + threadIdx.x % 8, lane = threadIdx.x / 8;
+  const float *p = partial + (e ? (int64_t)w.rows[0] * D : 0) + col;
+  float v = 0.f;
+#pragma unroll 8
+  for (int i = lane; i < w.rows[e]; i += 128) v += p[(int64_t)i * D];
+  sums[lane][threadIdx.x % 8] = v;
+  __syncthreads();
+  for (int n = 64; n >= 1; n /= 2) {
+    if (lane < n) sums[lane][threadIdx.x % 8] += sums[lane + n][threadIdx.x % 8];
+    __syncthreads();
+  }
+  if (lane == 0 && w.out[e]) {
+    if (f32) static_cast<float *>(w.out[e])[col] = sums[0][threadIdx.x];
+    else static_cast<T *>(w.out[e])[col] = T(sums[0][threadIdx.x]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+namespace {
+
+int lanes_per_row(int D) {
+  int n = 1;
+  while (n < D / 16) n *= 2;
+  return n;
+}
+
+int check_norm(const fa_norm_rotary_args *a) {
+  if (!a || (a->dtype != FA_F16 && a->dtype != FA_BF16)) return FA_ERR_BAD_ARG;
+  if (a->B < 0 || a->L < 0 || a->H <= 0 || a->Hk <= 0 || a->D <= 0 || a->table_rows <= 0 || a->rotary_dim < 0)
+    return FA_ERR_BAD_ARG;
+  if (!a->cos || !a->sin) return FA_ERR_BAD_ARG;
+  if (a->D % 16 || a->D > 512 || a->rotary_dim % 16 || a->rotary_dim > a->D) return FA_ERR_UNSUPPORTED;
+  if (!aligned16(a->cos) || !aligned16(a->sin) || !aligned16(a->q_weight) || !aligned16(a->k_weight))
+    return FA_ERR_ALIGNMENT;
+  return FA_OK;
+}
+
+// A CTA's heads: all that share a position's angles, but fewer where the grid would not be `waves` of 4 CTAs an SM.
+// (`tiles`: positions groups a CTA walks on top, where it would be deeper; for the backward, whose CTAs leave a row of
+// partial sums each.)
+int64_t plan_norm(const fa_norm_rotary_args *s, NormArgs *a, int waves, bool walk) {
+  const int rows = kNormThreads / lanes_per_row(s->D);
+  const int64_t positions = (int64_t)((s->L + rows - 1) / rows) * s->B, want = (int64_t)148 * 4 * waves;
+  const int all = s->H + s->Hk;
+  int per = 1;
+  while (per < all && positions * ((all + 2 * per - 1) / (2 * per)) >= want) per *= 2;
+  per = per > 8 ? 8 : per;
+  for (int e = 0; e < 2; ++e) {
+    const int heads = e ? s->Hk : s->H;
+    a->per_cta[e] = per < heads ? per : heads;
+    a->chunks[e] = (heads + a->per_cta[e] - 1) / a->per_cta[e];
+  }
+  const int Z = a->chunks[0] + a->chunks[1];
+  int tiles = 1;
+  const int64_t strips = (s->L + rows - 1) / rows;
+  while (walk && strips > tiles && (strips + 2 * tiles - 1) / (2 * tiles) * s->B * Z >= want) tiles *= 2;
+  a->tiles = tiles;
+  return (strips + tiles - 1) / tiles * s->B * Z;
+}
+
+void fill_norm(const fa_norm_rotary_args *s, NormArgs *a) {
+  a->cos = s->cos, a->sin = s->sin, a->positions = s->positions, a->pos_stride_b = s->pos_stride_b, a->eps = s->eps;
+  a->B = s->B, a->L = s->L, a->D = s->D, a->R = s->rotary_dim, a->table_rows = s->table_rows;
+  a->weight_is_f32 = s->weight_is_f32;
+  a->side[0].weight = s->q_weight, a->side[1].weight = s->k_weight;
+  a->side[0].heads = s->H, a->side[1].heads = s->Hk;
+}
+
+constexpr int kForwardWaves = 16, kBackwardWaves = 4;
+
+template <typename T, int LPR, bool IL>
+int launch_norm(const NormArgs &a, int64_t grid, bool backward, float *partial, cudaStream_t s) {
+  if (backward) qk_norm_rotary_bwd_kernel<T, LPR, IL><<<(unsigned)grid, kNormThreads, 0, s>>>(a, partial);
+  else qk_norm_rotary_fwd_kernel<T, LPR, IL><<<(unsigned)grid, kNormThreads, 0, s>>>(a);
+  FA_CHECK_LAUNCH();
+  return FA_OK;
+}
+template <typename T, bool IL>
+int dispatch_lanes(int D, const NormArgs &a, int64_t grid, bool backward, float *partial, cudaStream_t s) {
+  switch (lanes_per_row(D)) {
+    case 1: return launch_norm<T, 1, IL>(a, grid, backward, partial, s);
+    case 2: return launch_norm<T, 2, IL>(a, grid, backward, partial, s);
+    case 4: return launch_norm<T, 4, IL>(a, grid, backward, partial, s);
+    case 8: return launch_norm<T, 8, IL>(a, grid, backward, partial, s);
+    case 16: return launch_norm<T, 16, IL>(a, grid, backward, partial, s);
+    default: return launch_norm<T, 32, IL>(a, grid, backward, partial, s);
+  }
+}
+int dispatch_norm(const fa_norm_rotary_args *p, const NormArgs &a, int64_t grid, bool backward, float *partial,
+                  cudaStream_t s) {
+  if (grid >= (1ll << 31)) return FA_ERR_TOO_LARGE;
+  if (p->dtype == FA_F16)
+    return p->interleaved ? dispatch_lanes<__half, true>(p->D, a, grid, backward, partial, s)
+                          : dispatch_lanes<__half, false>(p->D, a, grid, backward, partial, s);
+  return p->interleaved ? dispatch_lanes<__nv_bfloat16, true>(p->D, a, grid, backward, partial, s)
+                        : dispatch_lanes<__nv_bfloat16, false>(p->D, a, grid, backward, partial, s);
+}
+
+}  // namespace
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" int fa_qk_norm_rotary_fwd(const fa_norm_rotary_args *p, const fa_tensor4 *q, const fa_tensor4 *k,
+                                     const fa_tensor4 *q_out, const fa_tensor4 *k_out, void *stream) {
+  if (int st = check_norm(p)) return st;
+  if (p->B == 0 || p->L == 0) return FA_OK;
+  for (const fa_tensor4 *t : {q, k, q_out, k_out}) {
+    if (!tensor_ok(t)) return FA_ERR_BAD_ARG;
+    if (!tensor_aligned(t)) return FA_ERR_ALIGNMENT;
+  }
+  NormArgs a{};
+  fill_norm(p, &a);
+  a.side[0].x = q->ptr, a.side[0].sx = strides_of(q), a.side[0].y = q_out->ptr, a.side[0].sy = strides_of(q_out);
+  a.side[1].x = k->ptr, a.side[1].sx = strides_of(k), a.side[1].y = k_out->ptr, a.side[1].sy = strides_of(k_out);
+  return dispatch_norm(p, a, plan_norm(p, &a, kForwardWaves, false), false, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t fa_qk_norm_rotary_bwd_workspace_bytes(const fa_norm_rotary_args *p) {
+  if (check_norm(p) || p->B == 0 || p->L == 0) return 0;
+  NormArgs a{};
+  return plan_norm(p, &a, kBackwardWaves, true) * p->D * 4;
+}
+
+extern "C" int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *p, const fa_tensor4 *q, const fa_tensor4 *k,
+                                     const fa_tensor4 *gq, const fa_tensor4 *gk, const fa_tensor4 *dq,
+                                     const fa_tensor4 *dk, void *dq_weight, void *dk_weight, void *workspace,
+                                     int64_t workspace_bytes, void *stream) {
+  if (int st = check_norm(p)) return st;
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool weights = dq_weight || dk_weight;
+  if (p->B == 0 || p->L == 0) {
+    const size_t bytes = (size_t)p->D * (p->weight_is_f32 ? 4 : 2);
+    for (void *w : {dq_weight, dk_weight})
+      if (w && cudaMemsetAsync(w, 0, bytes, s) != cudaSuccess) return FA_ERR_LAUNCH;
+    return FA_OK;
+  }
+  for (const fa_tensor4 *t : {q, k, gq, gk, dq, dk}) {
+    if (!tensor_ok(t)) return FA_ERR_BAD_ARG;
+    if (!tensor_aligned(t)) return FA_ERR_ALIGNMENT;
+  }
+  NormArgs a{};
+  fill_norm(p, &a);
+  const fa_tensor4 *xs[2] = {q, k}, *gs[2] = {gq, gk}, *ds[2] = {dq, dk};
+  for (int e = 0; e < 2; ++e) {
+    a.side[e].x = xs[e]->ptr, a.side[e].sx = strides_of(xs[e]);
+    a.side[e].g = gs[e]->ptr, a.side[e].sg = strides_of(gs[e]);
+    a.side[e].y = ds[e]->ptr, a.side[e].sy = strides_of(ds[e]);
+  }
+  const int64_t grid = plan_norm(p, &a, kBackwardWaves, true);
+  if (weights && (!workspace || !aligned16(workspace) || workspace_bytes < grid * p->D * 4)) return FA_ERR_WORKSPACE;
+  float *partial = weights ? static_cast<float *>(workspace) : nullptr;
+  if (int st = dispatch_norm(p, a, grid, true, partial, s)) return st;
+  if (!weights) return FA_OK;
+  const int64_t strips = grid / (a.chunks[0] + a.chunks[1]);
+  const WeightGrad w{{dq_weight, dk_weight}, {(int)(strips * a.chunks[0]), (int)(strips * a.chunks[1])}};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p->D / 8, 2), cfg.blockDim = dim3(1024), cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
+  const cudaError_t st =
+      p->dtype == FA_F16
+          ? cudaLaunchKernelEx(&cfg, weight_grad_kernel<__half>, (const float *)partial, w, (int)p->D, (int)p->weight_is_f32)
+          : cudaLaunchKernelEx(&cfg, weight_grad_kernel<__nv_bfloat16>, (const float *)partial, w, (int)p->D,
+                               (int)p->weight_is_f32);
+  if (st != cudaSuccess) return FA_ERR_LAUNCH;
+  FA_CHECK_LAUNCH();
+  return FA_OK;
+}

@@ -9,8 +9,9 @@ import functools
 import torch
 
 from . import _C, _native
+from .qk_norm import check_tables, check_weights
 
-__all__ = ["attention", "reshape_and_cache"]
+__all__ = ["attention", "attention_8bit", "reshape_and_cache", "rotary_and_cache"]
 
 
 def _next_power_of_2(n):
@@ -231,3 +232,170 @@ def reshape_and_cache(key, value, key_cache, value_cache, slot_mapping):
             value.data_ptr(), key.stride(0), key.stride(1), key_cache.data_ptr(), value_cache.data_ptr(), kb, kh, kt,
             slots.data_ptr(), _C.raw_stream(key.device))
     _C.check(st, "fa_paged_cache_append")
+
+
+# ---- caches of 8 bits --------------------------------------------------------------------------------------------------
+def _check_scales(key_cache, key_scales, value_scales):
+    for t in (key_scales, value_scales):
+        assert t.dtype == torch.float32 and t.shape == key_cache.shape[:2] and t.is_contiguous(), \
+            "scales are contiguous fp32 [num_blocks, kv_heads]"
+        assert t.device == key_cache.device, f"scales are on {t.device}, the caches on {key_cache.device}"
+
+
+def _check_caches(key_cache, value_cache, num_kv_heads, head_size, unit):
+    """What both writers and readers of caches with a table ask: `unit` elements are 16 bytes."""
+    assert key_cache.dim() == 4 and key_cache.shape == value_cache.shape
+    assert key_cache.shape[1] == num_kv_heads and key_cache.shape[3] == head_size
+    assert key_cache.dtype == value_cache.dtype
+    assert key_cache.device == value_cache.device, "the caches are on one device"
+    assert key_cache.stride() == value_cache.stride(), "key and value cache must share strides"
+    assert key_cache.stride(-1) == 1 and all(s % unit == 0 for s in key_cache.stride()[:-1]) \
+        and key_cache.data_ptr() % 16 == 0 and value_cache.data_ptr() % 16 == 0, \
+        "caches need unit inner stride and 16-byte aligned rows"
+
+
+def _table_ready(block_tables, num_seqs, device):
+    assert block_tables.dtype in (torch.int32, torch.int64) and block_tables.dim() == 2
+    assert block_tables.shape[0] == num_seqs and block_tables.device == device
+    return block_tables if block_tables.stride(1) == 1 or block_tables.shape[1] <= 1 else block_tables.contiguous()
+
+
+def _int32(t, name, n, device):
+    assert t.device == device, f"{name} is on {t.device}, the operands on {device}"
+    assert not t.is_floating_point() and t.shape == (n,), f"{name} has {n} integers"
+    return t.to(torch.int32).contiguous()
+
+
+def _rows_ready(t):
+    """Unit inner stride, 16-byte aligned rows."""
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
+        s % 8 == 0 or n <= 1 for n, s in zip(t.shape[:2], t.stride()[:2]))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _stride(t, i):
+    return t.stride(i) if t.shape[i] > 1 else 0
+
+
+def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
+                   max_context_len, num_splits=0):
+    """`attention` over caches held in 8 bits: key_cache, value_cache [num_blocks, kv_heads, block, head] of
+    torch.float8_e4m3fn, key_scales, value_scales [num_blocks, kv_heads] fp32, 0 or positive; a value is code * scale.
+
+    query [num_seqs, kv_heads * group, head] fp16 / bf16, head 16, 32, 64, 128 or 256; block a multiple of 16;
+    context_lens [num_seqs] and block_tables [num_seqs, max_blocks] as in `attention`.  A sequence of length 0 gives 0;
+    one whose table names a block that the cache does not have gives NaN.  fp32 sums and statistics, the output rounded
+    once.  `rotary_and_cache` writes such caches."""
+    assert query.dim() == 3
+    num_seqs, num_q_heads, head_size = query.shape
+    assert query.is_cuda, "query must be a CUDA tensor"
+    dtype = _C.dtype_code(query.dtype)
+    num_kv_heads, kv_block_size = key_cache.shape[1], key_cache.shape[2]
+    assert num_kv_heads > 0 and num_q_heads > 0 and num_q_heads % num_kv_heads == 0
+    assert head_size in (16, 32, 64, 128, 256), f"head_size={head_size}"
+    assert key_cache.dtype == torch.float8_e4m3fn, "caches of torch.float8_e4m3fn"
+    assert kv_block_size > 0 and kv_block_size % 16 == 0, f"kv_block_size={kv_block_size}"
+    assert key_cache.device == query.device, f"key_cache is on {key_cache.device}, query on {query.device}"
+    _check_caches(key_cache, value_cache, num_kv_heads, head_size, 16)
+    _check_scales(key_cache, key_scales, value_scales)
+    max_context_len = int(max_context_len)
+    assert max_context_len > 0 and num_splits >= 0
+    context_lens = _int32(context_lens, "context_lens", num_seqs, query.device)
+    block_tables = _table_ready(block_tables, num_seqs, query.device)
+    query = _rows_ready(query)
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if num_seqs == 0:
+        return out
+    with _C.device_guard(query.device):
+        partition_size, P, sizing = _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits,
+                                          _C.sm_count(query.device))
+        part_out = part_max = part_sum = 0
+        if partition_size:
+            assert partition_size % 16 == 0, f"partition_size={partition_size}"
+            ws, part_out, part_max, part_sum = partition_workspace(num_seqs * num_q_heads, P, head_size, query.device)
+        kb, kh, kt = key_cache.stride()[:3]
+        args = _C.PAGED_8BIT_ARGS.pack(
+            dtype, num_seqs, num_q_heads, num_kv_heads, head_size, kv_block_size, max_context_len,
+            1 if block_tables.dtype == torch.int64 else 0, partition_size, attn_scale, query.data_ptr(),
+            _stride(query, 0), _stride(query, 1), key_cache.data_ptr(), value_cache.data_ptr(), kb, kh, kt,
+            context_lens.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), out.data_ptr(), out.stride(0),
+            out.stride(1), part_out, part_max, part_sum, 0, key_scales.data_ptr(), value_scales.data_ptr(),
+            key_cache.shape[0], block_tables.shape[1])
+        st = _C.call("fa_paged_attention_8bit")(args, *(sizing or (0, 0, 0, 0)), _C.raw_stream(query.device))
+    _C.check(st, "fa_paged_attention_8bit")
+    return out
+
+
+def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, block_tables, cos, sin, query_starts=None,
+                     positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, key_scales=None,
+                     value_scales=None):
+    """Writes the new tokens of a batch of sequences into the paged caches, keys rotated (and normed) on the way, and
+    returns their queries rotated (and normed): the step in front of `attention` or `attention_8bit`.
+
+    query [num_tokens, heads, head], key, value [num_tokens, kv_heads, head], fp16 / bf16, head 16, 32, 64, 128 or 256.
+    context_lens [num_seqs] counts the new tokens, as the attention that follows takes it; sequence s has rows
+    query_starts[s] .. query_starts[s + 1] - 1 (integers [num_seqs + 1], ascending), the last of them its last token; None: one
+    row a sequence.  block_tables [num_seqs, max_blocks].  A row's position in the tables is its place in its sequence,
+    or positions [num_tokens], clamped to them.  cos, sin, weights, eps, interleaved: as in qk_norm_rotary, no norm
+    without weights.
+
+    Caches [num_blocks, kv_heads, block, head] of the operands' type, or of torch.float8_e4m3fn with key_scales,
+    value_scales [num_blocks, kv_heads] fp32: a block's scale starts with its first token, is the least power of two
+    that holds its values, and earlier codes are brought along when it grows, so that a block filled token by token is one
+    filled at once (but for codes below 2^-6, which lose bits on the way).  Infinities are held as +-448 times the scale.
+
+    Rows behind the last sequence, or in front of theirs (context_lens smaller than its rows; 0 for an idle slot of a
+    padded batch), are written nowhere and come back as 0.  A block that is written to must belong to one sequence only:
+    otherwise what its places hold afterwards is not defined."""
+    assert query.dim() == key.dim() == value.dim() == 3
+    num_tokens, num_q_heads, head_size = query.shape
+    num_kv_heads = key.shape[1]
+    assert value.shape == key.shape and key.shape[0] == num_tokens and key.shape[2] == head_size
+    assert query.is_cuda, "query must be a CUDA tensor"
+    dtype = _C.dtype_code(query.dtype)
+    assert query.dtype == key.dtype == value.dtype
+    assert num_q_heads > 0 and num_kv_heads > 0
+    assert head_size in (16, 32, 64, 128, 256), f"head_size={head_size}"
+    device = query.device
+    for name, t in (("key", key), ("value", value), ("key_cache", key_cache)):
+        assert t.device == device, f"{name} is on {t.device}, query on {device}"
+    held = key_cache.dtype == torch.float8_e4m3fn
+    assert held or key_cache.dtype == query.dtype, "caches of the operands' type or of torch.float8_e4m3fn"
+    assert (key_scales is not None) == (value_scales is not None) == held, "scales belong to caches of 8 bits"
+    _check_caches(key_cache, value_cache, num_kv_heads, head_size, 16 if held else 8)
+    assert key_cache.shape[2] > 0
+    if held:
+        _check_scales(key_cache, key_scales, value_scales)
+    num_seqs = context_lens.shape[0]
+    context_lens = _int32(context_lens, "context_lens", num_seqs, device)
+    block_tables = _table_ready(block_tables, num_seqs, device)
+    assert query_starts is not None or num_tokens == num_seqs, "one row a sequence, or query_starts"
+    if query_starts is not None:
+        query_starts = _int32(query_starts, "query_starts", num_seqs + 1, device)
+    if positions is not None:
+        assert not positions.is_floating_point() and positions.shape == (num_tokens,), "positions are num_tokens integers"
+        assert positions.device == device, f"positions are on {positions.device}, query on {device}"
+        positions = positions.to(torch.int64).contiguous()
+    cos, sin = check_tables(cos, sin, head_size, device)
+    q_weight, k_weight = check_weights(q_weight, k_weight, head_size, query)
+    query, key, value = _rows_ready(query), _rows_ready(key), _rows_ready(value)
+    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if num_tokens == 0:
+        return out
+
+    def ptr(t):
+        return 0 if t is None else t.data_ptr()
+
+    kb, kh, kt = key_cache.stride()[:3]
+    args = _C.ROTARY_CACHE_ARGS.pack(
+        dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size, 2 * cos.shape[1], 1 if interleaved else 0,
+        key_cache.shape[2], key_cache.shape[0], block_tables.shape[1], 1 if block_tables.dtype == torch.int64 else 0,
+        cos.shape[0], 1 if q_weight is not None and q_weight.dtype == torch.float32 else 0, eps,
+        *(x for t in (query, key, value, out) for x in (t.data_ptr(), _stride(t, 0), _stride(t, 1))),
+        key_cache.data_ptr(), value_cache.data_ptr(), kb, kh, kt, ptr(key_scales), ptr(value_scales),
+        context_lens.data_ptr(), ptr(query_starts), block_tables.data_ptr(), block_tables.stride(0), ptr(positions),
+        cos.data_ptr(), sin.data_ptr(), ptr(q_weight), ptr(k_weight))
+    with _C.device_guard(device):
+        st = _C.call("fa_rotary_cache")(args, _C.raw_stream(device))
+    _C.check(st, "fa_rotary_cache")
+    return out

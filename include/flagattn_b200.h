@@ -402,6 +402,90 @@ int fa_rotary_pair_bwd(int32_t dtype, int32_t B, int32_t H, int32_t L, int32_t D
                        int64_t pos_stride_b, const fa_tensor4 *dx, void *stream);
 
 /* ---------------------------------------------------------------------- */
+/* Norm and rotation of queries and keys; the paged cache's fused writer     */
+/* and the decode over a cache of 8 bits (no counterpart in the reference)   */
+/* ---------------------------------------------------------------------- */
+
+/* RMS norm of every head of q (B, H, L, D) and k (B, Hk, L, D) and the rotation by position:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight;  y = n with its first `rotary_dim` elements rotated,
+ * pairs (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1), by row p of the tables as in
+ * fa_rotary_pair_fwd.  Tables: fp32, `table_rows` rows of rotary_dim / 2 values, contiguous.  Weights: D
+ * values of the 16-bit type or, weight_is_f32, of fp32; NULL = ones.  positions as in
+ * fa_rotary_pair_fwd.  D a multiple of 16, at most 512; rotary_dim a multiple of 16, at most D.
+ * fp32 throughout, each result rounded once. */
+typedef struct fa_norm_rotary_args {
+  int32_t dtype, B, H, Hk, L, D, rotary_dim, interleaved, weight_is_f32, table_rows;
+  float eps;
+  const void *q_weight, *k_weight;
+  const float *cos, *sin;
+  const int64_t *positions;
+  int64_t pos_stride_b;
+} fa_norm_rotary_args;
+int fa_qk_norm_rotary_fwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, const fa_tensor4 *k,
+                          const fa_tensor4 *q_out, const fa_tensor4 *k_out, void *stream);
+/* Its backward from q, k and the gradients gq, gk of the results: dq, dk, and dq_weight, dk_weight (of the
+ * weights' type; NULL = not wanted).  The weights' gradients go by a workspace of
+ * fa_qk_norm_rotary_bwd_workspace_bytes (not needed where both are NULL) and are added in an order that depends on
+ * the shape alone. */
+int64_t fa_qk_norm_rotary_bwd_workspace_bytes(const fa_norm_rotary_args *a);
+int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, const fa_tensor4 *k, const fa_tensor4 *gq,
+                          const fa_tensor4 *gk, const fa_tensor4 *dq, const fa_tensor4 *dk, void *dq_weight,
+                          void *dk_weight, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The new tokens of a batch of sequences into the paged caches: query (num_tokens, q heads, head), key and value
+ * (num_tokens, kv heads, head) with strides of their own; every query and key head is normed (weights NULL: not)
+ * and rotated as above, queries go to `out`, keys and values to their places.
+ *   Sequence s has the rows [query_starts[s], query_starts[s + 1]) (NULL: row s alone, num_tokens == num_seqs), the
+ * last of which is token context_lens[s] - 1 of the sequence: lengths count the new tokens, as the attention that
+ * follows wants them.  A token's place is position place % block_size of block block_tables[s, place / block_size],
+ * its angle's row positions[row] or its place.  Rows of no sequence, rows in front of their sequence (more
+ * rows than tokens) and rows behind the table's columns are written nowhere and have 0 in `out`; a block id outside
+ * [0, num_blocks) is not written to.  A block that is written to belongs to one sequence.
+ *   key_scales, value_scales NULL: caches of the 16-bit type.  Otherwise e4m3 codes and fp32 scales
+ * (num_blocks, kv heads), contiguous: with 2^e the least power of two such that the finite new values of the block and
+ * head are at most 448 * 2^e (e >= -126), the scale becomes 2^e where the block's first token is among them, else
+ * max(scale, 2^e); codes of earlier tokens are brought to it, and new ones are the nearest to value / scale (infinities:
+ * +-448, NaN: NaN), from 64-bit arithmetic.
+ * head 16, 32, 64, 128 or 256; cache strides multiples of 8 (16-bit) or 16 (e4m3) elements. */
+typedef struct fa_rotary_cache_args {
+  int32_t dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size, rotary_dim, interleaved;
+  int32_t block_size, num_blocks, table_cols, block_table_is_i64, table_rows, weight_is_f32;
+  float eps;
+  const void *query;
+  int64_t q_stride_t, q_stride_h;
+  const void *key;
+  int64_t k_stride_t, k_stride_h;
+  const void *value;
+  int64_t v_stride_t, v_stride_h;
+  void *out;
+  int64_t o_stride_t, o_stride_h;
+  void *key_cache, *value_cache;
+  int64_t kv_stride_b, kv_stride_h, kv_stride_t;
+  float *key_scales, *value_scales;
+  const int32_t *context_lens, *query_starts;
+  const void *block_tables;
+  int64_t bt_stride_s;
+  const int64_t *positions;
+  const float *cos, *sin;
+  const void *q_weight, *k_weight;
+} fa_rotary_cache_args;
+int fa_rotary_cache(const fa_rotary_cache_args *a, void *stream);
+
+/* fa_paged_decode over caches of e4m3 codes (strides in codes, multiples of 16) with fp32 scales (num_blocks,
+ * num_kv_heads), contiguous, 0 or positive: value = code * scale.  `paged` as for fa_paged_decode, with
+ * block_size a multiple of 16, causal_rows 0 and a block table of `table_cols` columns.  partition_size 0: one
+ * pass; otherwise partial results in the workspace and their reduction, with partitions of partition_size tokens
+ * (finest 0) or sized on the GPU as in fa_paged_attention.  A block id outside [0, num_blocks) makes its sequence's
+ * output NaN. */
+typedef struct fa_paged_8bit_args {
+  fa_paged_args paged;
+  const float *key_scales, *value_scales;
+  int32_t num_blocks, table_cols;
+} fa_paged_8bit_args;
+int fa_paged_attention_8bit(const fa_paged_8bit_args *a, int32_t finest, int32_t coarsest, int32_t ctas, int32_t parts,
+                            void *stream);
+
+/* ---------------------------------------------------------------------- */
 /* Health check of the tensor-core kernels. Every wait inside them is bounded
  * (about a second); a wait that runs out stores a code naming the wait in a
  * per-device status word, and the kernel tears down and returns instead of
