@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -523,6 +524,264 @@ bool append(const Tensor &key, const Tensor &value, const Tensor &kc, const Tens
   return true;
 }
 
+// ---- qk_norm_rotary, rotary_and_cache, paged_attention_8bit ------------------------------------------------------------
+bool vector_ready(const Tensor &t) { return t.is_contiguous() && aligned16(t); }
+// fp32 (positions, half of the rotated elements), as the kernels read them
+bool angles_ready(const Tensor &cos, const Tensor &sin, int64_t D, int device) {
+  for (const Tensor *t : {&cos, &sin})
+    if (!plain(*t, device) || t->scalar_type() != at::kFloat || t->dim() != 2 || !fits(*t) || !vector_ready(*t) ||
+        t->requires_grad())
+      return false;
+  return cos.sizes() == sin.sizes() && 2 * cos.size(1) <= D && cos.size(1) % 8 == 0;
+}
+// both weights or neither, of one type
+bool weights_ready(const Tensor &qw, const Tensor &kw, int64_t D, const Tensor &like, int device) {
+  if (!qw.defined() && !kw.defined()) return true;
+  if (!qw.defined() || !kw.defined() || qw.scalar_type() != kw.scalar_type()) return false;
+  for (const Tensor *t : {&qw, &kw})
+    if (!plain(*t, device) || t->dim() != 1 || t->size(0) != D || !vector_ready(*t) ||
+        (t->scalar_type() != at::kFloat && t->scalar_type() != like.scalar_type()))
+      return false;
+  return true;
+}
+const void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// the layout of `t` where that suits the kernels
+Tensor new_in_layout(const Tensor &t) {
+  Tensor y = at::empty_like(t);
+  return kernel_ready(y) ? y : new_like(t);
+}
+
+struct NormCall {   // operands in the kernels' layout; weights and positions may be undefined
+  Tensor q, k, qw, kw, cos, sin, positions;
+  bool interleaved;
+  double eps;
+  fa_norm_rotary_args args() const {
+    fa_norm_rotary_args a{};
+    dtype_code(q, &a.dtype);
+    a.B = (int32_t)q.size(0), a.H = (int32_t)q.size(1), a.Hk = (int32_t)k.size(1), a.L = (int32_t)q.size(2);
+    a.D = (int32_t)q.size(3), a.rotary_dim = (int32_t)(2 * cos.size(1)), a.interleaved = interleaved;
+    a.weight_is_f32 = qw.defined() && qw.scalar_type() == at::kFloat, a.table_rows = (int32_t)cos.size(0);
+    a.eps = (float)eps, a.q_weight = ptr(qw), a.k_weight = ptr(kw);
+    a.cos = cos.data_ptr<float>(), a.sin = sin.data_ptr<float>();
+    if (positions.defined()) {
+      a.positions = positions.data_ptr<int64_t>();
+      a.pos_stride_b = positions.dim() > 1 && positions.size(0) > 1 ? positions.size(1) : 0;
+    }
+    return a;
+  }
+  variable_list forward() const {
+    Tensor q_out = new_in_layout(q), k_out = new_in_layout(k);
+    const fa_norm_rotary_args a = args();
+    const fa_tensor4 tq = tensor4(q), tk = tensor4(k), oq = tensor4(q_out), ok = tensor4(k_out);
+    check(fa_qk_norm_rotary_fwd(&a, &tq, &tk, &oq, &ok, stream_of(q)), "fa_qk_norm_rotary_fwd");
+    return {q_out, k_out};
+  }
+};
+
+struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &, const Tensor &, const std::optional<Tensor> &,
+                               const std::optional<Tensor> &, const NormCall *c) {
+    variable_list out = c->forward();
+    ctx->save_for_backward({c->q, c->k, c->qw, c->kw, c->cos, c->sin, c->positions});
+    ctx->saved_data["interleaved"] = c->interleaved;
+    ctx->saved_data["eps"] = c->eps;
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const NormCall c{t[0], t[1], t[2], t[3], t[4], t[5], t[6], ctx->saved_data["interleaved"].toBool(),
+                     ctx->saved_data["eps"].toDouble()};
+    const bool graph = at::GradMode::is_enabled();
+    variable_list out(5);
+    {
+      at::AutoGradMode no_graph(false);
+      const c10::cuda::CUDAGuard guard(c.q.device());
+      const Tensor gq = ready(grads[0]), gk = ready(grads[1]);
+      out[0] = new_in_layout(c.q), out[1] = new_in_layout(c.k);
+      Tensor ws;
+      int64_t bytes = 0;
+      const fa_norm_rotary_args a = c.args();
+      if (c.qw.defined()) {
+        for (int i = 0; i < 2; ++i)
+          if (ctx->needs_input_grad(2 + i)) out[2 + i] = at::empty(c.qw.sizes(), c.qw.options());
+        if (out[2].defined() || out[3].defined()) {
+          bytes = fa_qk_norm_rotary_bwd_workspace_bytes(&a);
+          ws = at::empty({bytes}, c.q.options().dtype(at::kByte));
+        }
+      }
+      const fa_tensor4 tq = tensor4(c.q), tk = tensor4(c.k), tgq = tensor4(gq), tgk = tensor4(gk), tdq = tensor4(out[0]),
+                       tdk = tensor4(out[1]);
+      check(fa_qk_norm_rotary_bwd(&a, &tq, &tk, &tgq, &tgk, &tdq, &tdk, const_cast<void *>(ptr(out[2])),
+                                  const_cast<void *>(ptr(out[3])), const_cast<void *>(ptr(ws)), bytes, stream_of(c.q)),
+            "fa_qk_norm_rotary_bwd");
+    }
+    if (graph) {   // as torch's once_differentiable: an error for whoever goes through these gradients again
+      variable_list given;
+      for (Tensor &x : out)
+        if (x.defined()) given.push_back(x.detach().set_requires_grad(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>("qk_norm_rotary is differentiable once",
+                                                                   (int64_t)given.size());
+      variable_list marked = (*error)(std::move(given));
+      size_t i = 0;
+      for (Tensor &x : out)
+        if (x.defined()) x = marked[i++];
+    }
+    return out;
+  }
+};
+
+variable_list qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &qw, const Tensor &kw, const Tensor &cos,
+                             const Tensor &sin, const Tensor &positions, bool interleaved, double eps) {
+  if (!q.is_cuda() || !usual_surroundings()) return {};
+  const int device = c10::cuda::current_device();
+  int32_t code;
+  if (!plain(q, device) || !plain(k, device) || q.dim() != 4 || k.dim() != 4 || !fits(q) || !fits(k) ||
+      !dtype_code(q, &code) || k.scalar_type() != q.scalar_type())
+    return {};
+  const int64_t B = q.size(0), L = q.size(2), D = q.size(3);
+  if (D % 16 != 0 || D > 512 || k.size(0) != B || k.size(2) != L || k.size(3) != D) return {};
+  if (!angles_ready(cos, sin, D, device) || !weights_ready(qw, kw, D, q, device)) return {};
+  NormCall c{q, k, qw, kw, cos, sin, positions, interleaved, eps};
+  if (positions.defined()) {
+    if (!plain(positions, device) || !integers(positions) || positions.dim() < 1 || positions.dim() > 2 ||
+        positions.size(-1) != L || (positions.dim() == 2 && positions.size(0) != 1 && positions.size(0) != B))
+      return {};
+    c.positions = positions.to(at::kLong).contiguous();
+  }
+  const bool weights_grad = qw.defined() && (qw.requires_grad() || kw.requires_grad());
+  const bool grads = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || weights_grad);
+  if (!kernel_ready(q) || !kernel_ready(k)) {
+    at::AutoGradMode no_graph(false);
+    c.q = ready(q), c.k = ready(k);
+    if (!kernel_ready(c.q) || !kernel_ready(c.k)) return {};
+  }
+  if (!grads) {
+    at::AutoGradMode no_graph(false);
+    return c.forward();
+  }
+  const auto some = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+  return QkNormRotary::apply(q, k, some(qw), some(kw), static_cast<const NormCall *>(&c));
+}
+
+// a pair of caches with a block table: as the kernels read them, `unit` elements 16 bytes
+bool tables_ready(const Tensor &kc, const Tensor &vc, int64_t Hk, int64_t D, int64_t unit, int device) {
+  if (!plain(kc, device) || !plain(vc, device) || kc.dim() != 4 || kc.sizes() != vc.sizes() || !fits(kc) ||
+      kc.strides() != vc.strides() || kc.scalar_type() != vc.scalar_type() || kc.size(1) != Hk || kc.size(3) != D ||
+      kc.stride(3) != 1 || !aligned16(kc) || !aligned16(vc))
+    return false;
+  return kc.stride(0) % unit == 0 && kc.stride(1) % unit == 0 && kc.stride(2) % unit == 0;
+}
+bool scales_ready(const Tensor &s, const Tensor &kc, int device) {
+  return plain(s, device) && s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == kc.size(0) &&
+         s.size(1) == kc.size(1) && s.is_contiguous();
+}
+bool lengths_ready(const Tensor &t, int64_t n, int device) {
+  return plain(t, device) && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+bool block_table_ready(const Tensor &t, int64_t seqs, int device) {
+  return plain(t, device) && integers(t) && t.dim() == 2 && t.size(0) == seqs && t.size(1) <= INT_MAX &&
+         (t.stride(1) == 1 || t.size(1) <= 1);
+}
+int64_t stride(const Tensor &t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; }
+// rows_ready() that does not ask for the strides of a size of one
+bool heads_ready(const Tensor &t) {
+  return t.stride(2) == 1 && aligned16(t) && stride(t, 0) % 8 == 0 && stride(t, 1) % 8 == 0;
+}
+
+// query, key, value, key_cache, value_cache, context_lens, block_tables, cos, sin; query_starts, positions, q_weight,
+// k_weight, key_scales, value_scales, which may be undefined
+Tensor rotary_and_cache(const Tensor *const (&t)[9], const Tensor (&o)[6], double eps, bool interleaved) {
+  const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &kc = *t[3], &vc = *t[4], &lens = *t[5], &table = *t[6], &cos = *t[7],
+               &sin = *t[8], &starts = o[0], &positions = o[1], &qw = o[2], &kw = o[3], &ks = o[4], &vs = o[5];
+  if (!q.is_cuda() || !usual_surroundings()) return {};
+  const int device = c10::cuda::current_device();
+  int32_t code;
+  for (const Tensor *x : {&q, &k, &v})
+    if (!plain(*x, device) || x->dim() != 3 || !fits(*x) || x->scalar_type() != q.scalar_type() || !heads_ready(*x)) return {};
+  const int64_t T = q.size(0), D = q.size(2), Hk = k.size(1);
+  if (!dtype_code(q, &code) || k.sizes() != v.sizes() || k.size(0) != T || k.size(2) != D) return {};
+  if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return {};
+  const bool held = ks.defined();
+  if (held != vs.defined() || !tables_ready(kc, vc, Hk, D, held ? 16 : 8, device) ||
+      kc.scalar_type() != (held ? at::kFloat8_e4m3fn : q.scalar_type()))
+    return {};
+  if (held && (!scales_ready(ks, kc, device) || !scales_ready(vs, kc, device))) return {};
+  if (!plain(lens, device) || lens.dim() != 1) return {};
+  const int64_t seqs = lens.size(0);
+  if (!lengths_ready(lens, seqs, device) || !block_table_ready(table, seqs, device)) return {};
+  if (starts.defined() ? !lengths_ready(starts, seqs + 1, device) : seqs != T) return {};
+  if (positions.defined() && (!plain(positions, device) || positions.scalar_type() != at::kLong || positions.dim() != 1 ||
+                              positions.size(0) != T || !positions.is_contiguous()))
+    return {};
+  if (!angles_ready(cos, sin, D, device) || !weights_ready(qw, kw, D, q, device)) return {};
+  at::AutoGradMode no_graph(false);
+  Tensor out = new_like(q);
+  fa_rotary_cache_args a{};
+  a.dtype = code, a.num_tokens = (int32_t)T, a.num_seqs = (int32_t)seqs, a.num_q_heads = (int32_t)q.size(1);
+  a.num_kv_heads = (int32_t)Hk, a.head_size = (int32_t)D, a.rotary_dim = (int32_t)(2 * cos.size(1));
+  a.interleaved = interleaved, a.block_size = (int32_t)kc.size(2), a.num_blocks = (int32_t)kc.size(0);
+  a.table_cols = (int32_t)table.size(1), a.block_table_is_i64 = table.scalar_type() == at::kLong;
+  a.table_rows = (int32_t)cos.size(0), a.weight_is_f32 = qw.defined() && qw.scalar_type() == at::kFloat;
+  a.eps = (float)eps;
+  a.query = q.data_ptr(), a.q_stride_t = stride(q, 0), a.q_stride_h = stride(q, 1);
+  a.key = k.data_ptr(), a.k_stride_t = stride(k, 0), a.k_stride_h = stride(k, 1);
+  a.value = v.data_ptr(), a.v_stride_t = stride(v, 0), a.v_stride_h = stride(v, 1);
+  a.out = out.data_ptr(), a.o_stride_t = stride(out, 0), a.o_stride_h = stride(out, 1);
+  a.key_cache = kc.data_ptr(), a.value_cache = vc.data_ptr();
+  a.kv_stride_b = kc.stride(0), a.kv_stride_h = kc.stride(1), a.kv_stride_t = kc.stride(2);
+  if (held) a.key_scales = ks.data_ptr<float>(), a.value_scales = vs.data_ptr<float>();
+  a.context_lens = lens.data_ptr<int32_t>(), a.query_starts = static_cast<const int32_t *>(ptr(starts));
+  a.block_tables = table.data_ptr(), a.bt_stride_s = table.stride(0);
+  a.positions = static_cast<const int64_t *>(ptr(positions));
+  a.cos = cos.data_ptr<float>(), a.sin = sin.data_ptr<float>(), a.q_weight = ptr(qw), a.k_weight = ptr(kw);
+  check(fa_rotary_cache(&a, stream_of(q)), "fa_rotary_cache");
+  return out;
+}
+
+// `P`: partitions of the workspace, 0 for one pass
+Tensor paged_8bit(const Tensor *const (&t)[7], double scale, int64_t most, int64_t partition, int64_t P,
+                  const int64_t (&sizing)[4]) {
+  const Tensor &q = *t[0], &kc = *t[1], &vc = *t[2], &ks = *t[3], &vs = *t[4], &lens = *t[5], &table = *t[6];
+  if (!q.is_cuda() || !usual_surroundings()) return {};
+  const int device = c10::cuda::current_device();
+  int32_t code;
+  if (!plain(q, device) || q.dim() != 3 || !fits(q) || !dtype_code(q, &code) || !heads_ready(q) || kc.dim() != 4) return {};
+  const int64_t seqs = q.size(0), H = q.size(1), D = q.size(2), Hk = kc.size(1), block = kc.size(2);
+  if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return {};
+  if (!tables_ready(kc, vc, Hk, D, 16, device) || kc.scalar_type() != at::kFloat8_e4m3fn || H % Hk != 0 || block % 16 != 0)
+    return {};
+  if (!scales_ready(ks, kc, device) || !scales_ready(vs, kc, device) || !lengths_ready(lens, seqs, device) ||
+      !block_table_ready(table, seqs, device) || most > INT_MAX || partition % 16 != 0)
+    return {};
+  at::AutoGradMode no_graph(false);
+  Tensor out = new_like(q), ws;
+  fa_paged_8bit_args p{};
+  fa_paged_args &a = p.paged;
+  a.dtype = code;
+  a.num_seqs = (int32_t)seqs, a.num_q_heads = (int32_t)H, a.num_kv_heads = (int32_t)Hk, a.head_size = (int32_t)D;
+  a.block_size = (int32_t)block, a.max_context_len = (int32_t)most;
+  a.block_table_is_i64 = table.scalar_type() == at::kLong, a.partition_size = (int32_t)partition;
+  a.attn_scale = (float)scale;
+  a.query = q.data_ptr(), a.q_stride_s = stride(q, 0), a.q_stride_h = stride(q, 1);
+  a.key_cache = kc.data_ptr(), a.value_cache = vc.data_ptr();
+  a.kv_stride_b = kc.stride(0), a.kv_stride_h = kc.stride(1), a.kv_stride_t = kc.stride(2);
+  a.context_lens = lens.data_ptr<int32_t>(), a.block_tables = table.data_ptr(), a.bt_stride_s = table.stride(0);
+  a.out = out.data_ptr(), a.o_stride_s = out.stride(0), a.o_stride_h = out.stride(1);
+  p.key_scales = ks.data_ptr<float>(), p.value_scales = vs.data_ptr<float>();
+  p.num_blocks = (int32_t)kc.size(0), p.table_cols = (int32_t)table.size(1);
+  if (partition) {   // paged.partition_workspace()
+    const int64_t rows = seqs * H, stats = (rows * P + 63) / 64 * 64;
+    ws = at::empty({rows * P * D + 2 * stats}, q.options().dtype(at::kFloat));
+    a.part_out = ws.data_ptr<float>();
+    a.part_max = a.part_out + rows * P * D;
+    a.part_sum = a.part_max + stats;
+  }
+  check(fa_paged_attention_8bit(&p, (int32_t)sizing[0], (int32_t)sizing[1], (int32_t)sizing[2], (int32_t)sizing[3],
+                                stream_of(q)),
+        "fa_paged_attention_8bit");
+  return out;
+}
+
 // ---- Python ----------------------------------------------------------------------------------------------------------
 // Arguments that are not what the fast form takes (a missing tensor, a float where a count is due) are not errors here:
 // the Python form says what is wrong with them.
@@ -651,6 +910,83 @@ PyObject *py_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// tensors or None, which leaves an undefined one
+bool optional_tensors(PyObject *const *args, int n, Tensor *out) {
+  for (int i = 0; i < n; ++i) {
+    const Tensor *t;
+    if (args[i] == Py_None) continue;
+    if (!tensors(args + i, 1, &t)) return false;
+    out[i] = *t;
+  }
+  return true;
+}
+bool number(PyObject *o, double *out) {
+  bool is_default;
+  return scale_of(o, &is_default, out) && !is_default;
+}
+
+// (q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps): weights and positions may be None
+PyObject *py_qk_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *t[2], *angles[2];
+  Tensor w[2], positions;
+  bool interleaved;
+  double eps;
+  if (n != 9 || !tensors(args, 2, t) || !optional_tensors(args + 2, 2, w) || !tensors(args + 4, 2, angles) ||
+      !optional_tensors(args + 6, 1, &positions) || !truth(args[7], &interleaved) || !number(args[8], &eps))
+    Py_RETURN_NONE;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release release;
+    out = qk_norm_rotary(*t[0], *t[1], w[0], w[1], *angles[0], *angles[1], positions, interleaved, eps);
+  }
+  if (out.empty()) Py_RETURN_NONE;
+  PyObject *pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out[0]));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(out[1]));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// (query, key, value, key_cache, value_cache, context_lens, block_tables, cos, sin, query_starts, positions, q_weight,
+// k_weight, key_scales, value_scales, eps, interleaved): the six in front of eps may be None
+PyObject *py_rotary_and_cache(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *t[9];
+  Tensor o[6], out;
+  double eps;
+  bool interleaved;
+  if (n != 17 || !tensors(args, 9, t) || !optional_tensors(args + 9, 6, o) || !number(args[15], &eps) ||
+      !truth(args[16], &interleaved))
+    Py_RETURN_NONE;
+  {
+    pybind11::gil_scoped_release release;
+    out = rotary_and_cache(t, o, eps, interleaved);
+  }
+  return wrap_or_none(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, scale, max_context_len, partition,
+// partitions, finest, coarsest, ctas, parts)
+PyObject *py_paged_8bit(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *t[7];
+  double scale;
+  int64_t x[7];
+  if (n != 15 || !tensors(args, 7, t) || !number(args[7], &scale)) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i)
+    if (!integer(args[8 + i], &x[i])) Py_RETURN_NONE;
+  Tensor o;
+  {
+    pybind11::gil_scoped_release release;
+    o = paged_8bit(t, scale, x[0], x[1], x[2], {x[3], x[4], x[5], x[6]});
+  }
+  return wrap_or_none(o);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject *py_backward_mode(PyObject *, PyObject *mode) {
   const long m = PyLong_AsLong(mode);
   if (m == -1 && PyErr_Occurred()) return nullptr;
@@ -693,6 +1029,9 @@ PyMethodDef methods[] = {{"flash", FAST(py_flash<false>)},
                          {"rotary_pair", FAST(py_rotary_pair)},
                          {"paged", FAST(py_paged)},
                          {"append", FAST(py_append)},
+                         {"qk_norm_rotary", FAST(py_qk_norm_rotary)},
+                         {"rotary_and_cache", FAST(py_rotary_and_cache)},
+                         {"paged_8bit", FAST(py_paged_8bit)},
                          {"coarsen_partition", FAST(py_coarsen)},
                          {"kernel_ready", FAST(py_kernel_ready)},
                          {"decode_covered", FAST(py_decode_covered)},

@@ -286,6 +286,11 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
     context_lens [num_seqs] and block_tables [num_seqs, max_blocks] as in `attention`.  A sequence of length 0 gives 0;
     one whose table names a block that the cache does not have gives NaN.  fp32 sums and statistics, the output rounded
     once.  `rotary_and_cache` writes such caches."""
+    if type(max_context_len) is int and max_context_len > 0 and num_splits == 0 and _native.usable(query):
+        out = _native_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
+                           max_context_len)
+        if out is not None:
+            return out
     assert query.dim() == 3
     num_seqs, num_q_heads, head_size = query.shape
     assert query.is_cuda, "query must be a CUDA tensor"
@@ -326,6 +331,21 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
     return out
 
 
+def _native_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
+                 max_context_len):
+    """The call through native code, or None; the partitions are chosen here."""
+    if query.dim() != 3 or key_cache.dim() != 4:
+        return None
+    num_seqs, num_q_heads, _ = query.shape
+    num_kv_heads, kv_block_size = key_cache.shape[1:3]
+    if not num_seqs or not num_q_heads or not num_kv_heads or num_q_heads % num_kv_heads or not kv_block_size:
+        return None
+    partition_size, P, sizing = _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, 0,
+                                      _C.sm_count(query.device))
+    return _native.load().paged_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
+                                     attn_scale, max_context_len, partition_size, P, *(sizing or (0, 0, 0, 0)))
+
+
 def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, block_tables, cos, sin, query_starts=None,
                      positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, key_scales=None,
                      value_scales=None):
@@ -347,6 +367,12 @@ def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, bl
     Rows behind the last sequence, or in front of theirs (context_lens smaller than its rows; 0 for an idle slot of a
     padded batch), are written nowhere and come back as 0.  A block that is written to must belong to one sequence only:
     otherwise what its places hold afterwards is not defined."""
+    if _native.usable(query):
+        out = _native.load().rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, block_tables, cos,
+                                              sin, query_starts, positions, q_weight, k_weight, key_scales, value_scales,
+                                              eps, interleaved)
+        if out is not None:
+            return out
     assert query.dim() == key.dim() == value.dim() == 3
     num_tokens, num_q_heads, head_size = query.shape
     num_kv_heads = key.shape[1]

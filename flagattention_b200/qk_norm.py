@@ -5,7 +5,6 @@ keys as they are.  One HBM-bound launch forward for q and k together; one backwa
 weights' gradients, in an order that depends on the shape alone.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C, _native, rotary
 
@@ -85,8 +84,17 @@ class QkNormRotary(torch.autograd.Function):
         return q_out, k_out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
+        with torch.no_grad():
+            grads = QkNormRotary._gradients(ctx, gq, gk)
+        if torch.is_grad_enabled():   # an error for whoever goes through these gradients again, with or without gq's graph
+            given = [g.detach().requires_grad_() for g in grads if g is not None]
+            marked = iter(torch._C._functions.DelayedError(b"qk_norm_rotary is differentiable once", len(given))(*given))
+            grads = [None if g is None else next(marked) for g in grads]
+        return (*grads, None, None, None, None, None)
+
+    @staticmethod
+    def _gradients(ctx, gq, gk):
         q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
         pos_stride, interleaved, eps = ctx.args
         gq, gk = _C.kernel_ready(gq), _C.kernel_ready(gk)
@@ -103,7 +111,7 @@ class QkNormRotary(torch.autograd.Function):
                 args, _C.pack4(q), _C.pack4(k), _C.pack4(gq), _C.pack4(gk), _C.pack4(dq), _C.pack4(dk), _ptr(dwq),
                 _ptr(dwk), _ptr(ws), size, _C.raw_stream(q.device))
         _C.check(st, "fa_qk_norm_rotary_bwd")
-        return dq, dk, dwq, dwk, None, None, None, None, None
+        return [dq, dk, dwq, dwk]
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, interleaved=False, eps=1e-6):
@@ -116,4 +124,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, interleav
     normed.  positions: None (token l sits at position l) or integers of shape (length,) or (batch, length); values outside
     the tables are clamped.  fp32 arithmetic, results rounded once.  Differentiable (once) with respect to q, k and the
     weights; the weights' gradients are the same bits every time."""
+    if _native.usable(q):
+        pair = _native.load().qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps)
+        if pair is not None:
+            return pair
     return QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps)
