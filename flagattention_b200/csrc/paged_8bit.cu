@@ -1,6 +1,6 @@
 // paged_attention_8bit decode: paged.cu's gather over a cache of e4m3 codes with an fp32 scale for each block and kv head.
 //
-// HBM-bound as there: every warp streams 32-token groups of codes and their scales through a cp.async ring of its own.
+// HBM-bound as there: every warp streams groups of codes and their scales through a cp.async ring of its own.
 // Codes go to fp16 (exactly) on the way from shared memory to the tensor cores, and two things follow from bytes:
 //  * S = Q K^T contracts over the head, in whatever order both operands agree on: a lane takes 16 codes that lie side by
 //    side as four steps of its K fragment, so K needs neither ldmatrix nor a transposition, and Q's fragments are read
@@ -29,9 +29,10 @@ constexpr float kLift = 6.f;
 template <int D>
 struct Paged8Cfg {
   static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
-  static constexpr int kWarps = D <= 128 ? 4 : 2;
-  static constexpr int kStages = D <= 64 ? 4 : 3;
-  static constexpr int kTokens = 32;                          // tokens of a group
+  static constexpr int kWarps = 4;
+  static constexpr int kStages = D <= 128 ? 4 : 3;
+  static constexpr int kTokens = 16;                          // tokens of a group
+  static constexpr int kCtas = D <= 128 ? 3 : 2;   // an SM: a fourth at 128 would spill (428 us for 64 x 1K-32K with 3, 565 with 4)
   static constexpr int kGroupBytes = kTokens * kD;            // of K or of V
   static constexpr int kStageBytes = 2 * kGroupBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -57,16 +58,6 @@ __device__ __forceinline__ constexpr uint32_t code_offset(int row, int piece) {
   return (uint32_t)(row * KD + 16 * (KD == 64 ? piece ^ (row & 2) : piece ^ (row & 7)));
 }
 
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
 // two e4m3 codes of a word, as two fp16 numbers
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
   uint32_t h;
@@ -91,7 +82,7 @@ __device__ __forceinline__ void split_scale(float scale, float &exponent, float 
 
 // HALF: at most 8 query rows, the upper half of the 16-row tile; the lower half serves the remainder of P.
 template <typename T, int D, typename IdxT, bool HALF>
-__global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
+__global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas)
     paged_8bit_kernel(const __grid_constant__ fa_paged_8bit_args p, const Sizing z) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the reduction waits for all of this grid by itself
   using C = Paged8Cfg<D>;
@@ -99,6 +90,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
   constexpr int R = HALF ? 1 : 2;   // accumulator rows of a thread: g and, in a full tile, g + 8
   constexpr int KJ = KD / 64;       // 16-byte pieces of a row that a lane of a quad takes for S
   constexpr int VW = KD / 32;       // 4-byte words of a row that a lane takes for O
+  constexpr int NT = GT / 8, NH = GT / 16;   // score fragments and 16-token pieces of a group
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const uint32_t smem = smem_u32(smem_raw);
   const fa_paged_args &a = p.paged;
@@ -137,19 +129,19 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
   const int bs_shift = (BS & (BS - 1)) == 0 ? 31 - __clz(BS) : -1;
 
   // A lane copies 16-byte piece `ch` of rows c * RPC + lane_r of a group, of K and of V.
-  constexpr int CPR = D / 16, RPC = 32 / CPR, NC = GT / RPC;
+  constexpr int CPR = D / 16, RPC = 32 / CPR, NC = (GT + RPC - 1) / RPC;
   const int lane_r = lane / CPR, ch = lane % CPR;
   uint32_t dst_off[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) dst_off[c] = code_offset<KD>(c * RPC + lane_r, ch);
   const int64_t lane_src = (int64_t)lane_r * a.kv_stride_t + ch * 16;
 
-  // blocks of the two halves of this warp's i-th group, looked up a group ahead of their use; -1 where the half holds no
-  // token of the partition, -2 for an id outside the cache
-  int64_t next[2];
+  // blocks of the 16-token pieces of this warp's i-th group, looked up a group ahead of their use; -1 where the piece
+  // holds no token of the partition, -2 for an id outside the cache
+  int64_t next[NH];
   auto look_up = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NH; ++s) {
       const int tok = t_begin + (warp + i * NW) * GT + 16 * s;
       next[s] = -1;
       if (i < my_groups && tok < t_end) {
@@ -158,33 +150,56 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
       }
     }
   };
+  const int64_t c_step = (int64_t)RPC * a.kv_stride_t;
   auto issue = [&](int i) {   // i-th group of this warp -> stage i % NS
     const int tok0 = t_begin + (warp + i * NW) * GT;
     const uint32_t st = ring + (i % NS) * C::kStageBytes;
-    const int64_t blk[2] = {next[0], next[1]};
-    look_up(i + 1);
-    const uint8_t *src[2];
+    int64_t blk[NH];
+    const uint8_t *src[NH];
+    bool whole = tok0 + GT <= t_end;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NH; ++s) {
+      blk[s] = next[s];
+      whole = whole && blk[s] >= 0;
       const int tok = tok0 + 16 * s;
       const int in_blk = bs_shift >= 0 ? tok & (BS - 1) : tok % BS;
-      // (the s-th half's rows are counted from the group's start)
-      src[s] = kc + max(blk[s], (int64_t)0) * a.kv_stride_b + (int64_t)(in_blk - 16 * s) * a.kv_stride_t + lane_src;
+      src[s] = kc + max(blk[s], (int64_t)0) * a.kv_stride_b + (int64_t)in_blk * a.kv_stride_t + lane_src;
     }
+    look_up(i + 1);
+    if (RPC <= 16 && whole) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int row = c * RPC + lane_r, s = row / 16;
-      const bool ok = tok0 + row < t_end && (s ? blk[1] : blk[0]) >= 0;
-      const uint8_t *sk = ok ? (s ? src[1] : src[0]) + (int64_t)(c * RPC) * a.kv_stride_t : kc;
-      cp_async16(st + dst_off[c], sk, ok);
-      cp_async16(st + C::kGroupBytes + dst_off[c], sk + v_minus_k, ok);
+      for (int c = 0; c < NC; ++c) {
+        const uint8_t *&from = src[c * RPC / 16];
+        cp_async16(st + dst_off[c], from, true);
+        cp_async16(st + C::kGroupBytes + dst_off[c], from + v_minus_k, true);
+        from += c_step;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int row = c * RPC + lane_r, s = row / 16;   // (a row of 16 bytes: a step covers both pieces)
+        const uint8_t *sk = kc;
+        bool ok = tok0 + row < t_end;
+#pragma unroll
+        for (int k = 0; k < NH; ++k)
+          if (s == k) {
+            ok = ok && blk[k] >= 0;
+            sk = src[k] + (int64_t)(RPC <= 16 ? c * RPC % 16 : -16 * k) * a.kv_stride_t;
+          }
+        if (s >= NH) ok = false;
+        if (!ok) sk = kc;
+        if (row < GT) {
+          cp_async16(st + dst_off[c], sk, ok);
+          cp_async16(st + C::kGroupBytes + dst_off[c], sk + v_minus_k, ok);
+        }
+      }
     }
-    if (lane < 4) {
+    if (lane < 2 * NH) {
       const uint32_t at = scales + (i % NS) * 16 + lane * 4;
-      const int64_t id = lane < 2 ? blk[0] : blk[1];
+      const int64_t id = blk[NH > 1 && lane >= 2 ? 1 : 0];
       const float *from = lane & 1 ? p.value_scales : p.key_scales;
       if (id >= 0) cp_async4(at, from + id * a.num_kv_heads + hk);
-      // a block outside the cache makes its sequence's output NaN; a half without tokens counts as nothing
+      // a block outside the cache makes its sequence's output NaN; a piece without tokens counts as nothing
       else asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(at), "f"(id == -2 ? NAN : 0.f) : "memory");
     }
   };
@@ -203,8 +218,9 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
 
   // ---- query group -> shared as fp16 (rows >= `rows` are zero) -----------------
   float *row_scale = reinterpret_cast<float *>(smem_raw + C::kRowScale);
-  {
-    constexpr int TPR = NW * 32 / 16, PIECES = KD / 8 / TPR;   // threads of a row, and their 8-element pieces
+  // threads of a row, and their 8-element pieces; whole warps
+  constexpr int TPR = NW * 2 < KD / 8 ? NW * 2 : KD / 8, PIECES = KD / 8 / TPR;
+  if (tid < 16 * TPR) {
     const int r = tid / TPR, t = tid % TPR;
     const T *q = static_cast<const T *>(a.query) + (int64_t)seq * a.q_stride_s + (int64_t)(qh0 + r) * a.q_stride_h;
     uint4 u[PIECES];
@@ -282,26 +298,28 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
 
     const int tok0 = t_begin + (warp + i * NW) * GT;
     const uint32_t st = ring + (i % NS) * C::kStageBytes, sv = st + C::kGroupBytes;
-    const uint4 sc = lds16(scales + (i % NS) * 16);
-    const float ks[2] = {__uint_as_float(sc.x), __uint_as_float(sc.z)};
-    float ve[2], vf[2];
-    split_scale(__uint_as_float(sc.y), ve[0], vf[0]);
-    split_scale(__uint_as_float(sc.w), ve[1], vf[1]);
-
-    float s[4][4];
+    float ks[NH], ve[NH], vf[NH];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int h = 0; h < NH; ++h) {
+      const uint2 sc = lds8(scales + (i % NS) * 16 + 8 * h);
+      ks[h] = __uint_as_float(sc.x);
+      split_scale(__uint_as_float(sc.y), ve[h], vf[h]);
+    }
+
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
-      uint4 k[4];
+      uint4 k[NT];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) k[n] = lds16(st + code_offset<KD>(8 * n + token_of<KD>(g), 4 * j + t4));
+      for (int n = 0; n < NT; ++n) k[n] = lds16(st + code_offset<KD>(8 * n + token_of<KD>(g), 4 * j + t4));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t qa[4];
         if (!kQInRegs) q_step(j, w, qa);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < NT; ++n) {
           const uint32_t kw = w == 0 ? k[n].x : w == 1 ? k[n].y : w == 2 ? k[n].z : k[n].w;
           Elem<__half>::mma(s[n], kQInRegs ? qf[4 * j + w] : qa, codes_lo(kw), codes_hi(kw));
         }
@@ -313,17 +331,21 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
     bool need = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float mx[2] = {-INFINITY, -INFINITY};   // of either half: they have scales of their own
+      float mx[NH];   // of each piece: they have scales of their own
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int h = 0; h < NH; ++h) mx[h] = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float &x = s[n][2 * r + e];
           x = tail && tok0 + 8 * n + col[e] >= t_end ? -INFINITY : x * (q_scale[r] * ks[n >> 1]);
           mx[n >> 1] = fmaxf(mx[n >> 1], x);
         }
-      m_new[r] = fmaxf(m_i[r], quad_max(fmaxf(mx[0], mx[1])));
-      w_new[r] = fmaxf(w_i[r], quad_max(fmaxf(mx[0] + ve[0], mx[1] + ve[1])));
+      float most = mx[0], most_w = mx[0] + ve[0];
+      if (NH > 1) most = fmaxf(most, mx[NH - 1]), most_w = fmaxf(most_w, mx[NH - 1] + ve[NH - 1]);
+      m_new[r] = fmaxf(m_i[r], quad_max(most));
+      w_new[r] = fmaxf(w_i[r], quad_max(most_w));
       // lazy, as in paged.cu: a reference moves when it is 2^8 behind
       need = need || m_new[r] - m_i[r] > 8.f || w_new[r] - w_i[r] > 8.f;
     }
@@ -343,21 +365,20 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32)
     for (int r = 0; r < R; ++r) {
       const float m_ref = m_i[r] == -INFINITY ? 0.f : m_i[r];   // all scores -inf: P = 0
       const float w_ref = w_i[r] == -INFINITY ? 0.f : w_i[r] - kLift;
-      const float shift[2] = {ve[0] - w_ref, ve[1] - w_ref};
       float rs = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float &x = s[n][2 * r + e];
           rs += fast_exp2(x - m_ref);
-          x = fast_exp2(x + shift[n >> 1]) * vf[n >> 1];
+          x = fast_exp2(x + (ve[n >> 1] - w_ref)) * vf[n >> 1];
         }
       l_i[r] += rs;
     }
     // P goes in as a 16-bit value and a 16-bit remainder, as in paged.cu
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {   // 16 tokens each
+    for (int h = 0; h < NH; ++h) {   // 16 tokens each
       uint32_t pa[4], pr[4];
       if (HALF) {
         split_weights<__half>(s[2 * h][0], s[2 * h][1], pa[0], pa[1]);

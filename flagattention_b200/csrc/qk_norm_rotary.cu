@@ -11,6 +11,7 @@
 // `kAhead` heads in flight; q and k share the launch (a small call is bound by launches), a CTA has heads of one of them.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "attn_params.cuh"
@@ -22,7 +23,8 @@ namespace fa {
 
 constexpr int kNormThreads = 128;
 constexpr int kAhead = 4;      // heads whose loads are in flight, forward
-constexpr int kAheadBwd = 2;   // backward: two tensors a head, and the sums of dw in registers
+constexpr int kForwardCtas = 5, kBackwardCtas = 4;   // resident on an SM
+constexpr int kRing = 3;     // backward: heads in flight and in work, 8 KB each
 
 struct NormSide {   // q or k
   const void *x, *g;
@@ -40,7 +42,7 @@ struct NormArgs {
   int B, L, D, R, table_rows, weight_is_f32;
   int per_cta[2];   // heads a CTA walks
   int chunks[2];    // and the CTAs that share a position's heads
-  int tiles;        // backward: groups of positions a CTA walks
+  int64_t items[2]; // backward: strips of positions x chunks, of q and of k
 };
 
 __device__ __forceinline__ uint4 load16(const void *p) { return *reinterpret_cast<const uint4 *>(p); }
@@ -58,12 +60,15 @@ struct NormLane {
   bool live;
   float c[8], s[8], wlo[8], whi[8];
 
-  __device__ __forceinline__ void place(const NormArgs &a) {
+  __device__ __forceinline__ void columns(const NormArgs &a) {
     const int j = threadIdx.x % LPR;
     const bool turns = j < a.R / 16;
     off_a = IL || !turns ? 16 * j : 8 * j;
     off_b = IL || !turns ? 16 * j + 8 : a.R / 2 + 8 * j;
     live = j < a.D / 16;
+  }
+  __device__ __forceinline__ void place(const NormArgs &a) {
+    columns(a);
     const int Z = a.chunks[0] + a.chunks[1];
     int z = blockIdx.x % Z;
     e = z >= a.chunks[0];
@@ -109,7 +114,7 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 template <typename T, int LPR, bool IL>
-__global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, kForwardCtas) qk_norm_rotary_fwd_kernel(const NormArgs a) {
   NormLane<T, LPR, IL> t;
   t.place(a);
   const int rows = kNormThreads / LPR;
@@ -121,21 +126,29 @@ __global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_fwd_kernel(con
   const T *x = static_cast<const T *>(side.x) + t.b * side.sx.b + (here ? t.l * side.sx.l : 0);
   T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0);
   const float inv_d = 1.f / a.D;
-
-  for (int h0 = t.h_lo; h0 < t.h_hi; h0 += kAhead) {
+  // the rotation and the weights in one: y_lo = r (x_lo ll - x_hi lh), y_hi = r (x_hi hh + x_lo hl)
+  float ll[8], lh[8], hh[8], hl[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    ll[i] = t.c[i] * t.wlo[i], hh[i] = t.c[i] * t.whi[i];
+    lh[i] = t.s[i] * t.whi[i], hl[i] = t.s[i] * t.wlo[i];
+  }
+  x += t.h_lo * side.sx.h;
+  y += t.h_lo * side.sy.h;
+  for (int left = t.h_hi - t.h_lo; left > 0; left -= kAhead) {
     uint4 ua[kAhead], ub[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
-      if (here && h0 + u < t.h_hi) {
-        const T *src = x + (int64_t)(h0 + u) * side.sx.h;
-        ua[u] = load16(src + t.off_a);
-        ub[u] = load16(src + t.off_b);
+      if (here && u < left) {
+        ua[u] = load16(x + t.off_a);
+        ub[u] = load16(x + t.off_b);
       }
+      x += side.sx.h;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (h0 + u >= t.h_hi) break;   // the same for the whole CTA
+      if (u >= left) break;   // the same for the whole CTA
       float va[8], vb[8], lo[8], hi[8], ylo[8], yhi[8];
       unpack8<T>(va, ua[u]);
       unpack8<T>(vb, ub[u]);
@@ -146,141 +159,182 @@ __global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_fwd_kernel(con
       to_pairs<IL>(lo, hi, va, vb);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float nl = lo[i] * r * t.wlo[i], nh = hi[i] * r * t.whi[i];
-        ylo[i] = nl * t.c[i] - nh * t.s[i];
-        yhi[i] = nh * t.c[i] + nl * t.s[i];
+        ylo[i] = (lo[i] * ll[i] - hi[i] * lh[i]) * r;
+        yhi[i] = (hi[i] * hh[i] + lo[i] * hl[i]) * r;
       }
       from_pairs<IL>(va, vb, ylo, yhi);
       if (here) {
-        T *dst = y + (int64_t)(h0 + u) * side.sy.h;
-        *reinterpret_cast<uint4 *>(dst + t.off_a) = pack8<T>(va);
-        *reinterpret_cast<uint4 *>(dst + t.off_b) = pack8<T>(vb);
+        *reinterpret_cast<uint4 *>(y + t.off_a) = pack8<T>(va);
+        *reinterpret_cast<uint4 *>(y + t.off_b) = pack8<T>(vb);
       }
+      y += side.sy.h;
     }
   }
 }
 
-// The rows of dw's partial sums, one a CTA of q or of k: partial[0 .. n_q) and [n_q .. n_q + n_k) of D floats, in an order
-// that depends on the shape alone, as do the sums: dw is the same bits every time.
+// Backward.  `ctas` CTAs take equal shares of the work items (a strip of positions, some heads of q or of k), those of q
+// first, and leave a row of dw's sums for q and one for k each: partial[0 .. ctas) and [ctas .. 2 ctas) of D floats.  Shares
+// and sums depend on the shape and the number of SMs alone: dw is the same bits every time.
+// x and g of a head go through a ring of asynchronous copies, kRing heads deep and across items, in which every thread
+// reads back what it asked for itself: no barrier, and loads in flight all the time, which registers had no room for.
+// B=2, H=32+8, L=4096, D=128 in bf16, forward and backward: 107 us with two heads' loads in registers and a row of sums
+// for each of 5120 CTAs (7 of them to add those up), 81 so (5200 GB/s); 4 CTAs an SM: a fifth spills, 96.
 template <typename T, int LPR, bool IL>
-__global__ void __launch_bounds__(kNormThreads, 4) qk_norm_rotary_bwd_kernel(const NormArgs a, float *partial) {
+__global__ void __launch_bounds__(kNormThreads, kBackwardCtas) qk_norm_rotary_bwd_kernel(const NormArgs a, float *partial) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the sum of the partial rows waits for all of this grid
   constexpr int kRows = kNormThreads / LPR, kWarps = kNormThreads / 32;
-  __shared__ float sums[kWarps][16 * LPR];
-  NormLane<T, LPR, IL> t;
-  t.place(a);
-  t.weights(a);
-  const int Z = a.chunks[0] + a.chunks[1];
-  const int first = (int)(blockIdx.x / ((unsigned)Z * a.B));
-  const NormSide &side = a.side[t.e];
+  __shared__ __align__(16) uint8_t ring[kRing * 4 * kNormThreads * 16];
+  float(*sums)[16 * LPR] = reinterpret_cast<float(*)[16 * LPR]>(ring);   // at the end of a side
+  static_assert(kWarps * 16 * LPR * 4 <= (int)sizeof(ring), "the sums go over the ring");
+  const uint32_t slot = smem_u32(ring) + threadIdx.x * 16;
   const float inv_d = 1.f / a.D;
-  float dlo[8], dhi[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) dlo[i] = dhi[i] = 0.f;
+  const int group = threadIdx.x / LPR;
 
-  for (int tile = 0; tile < a.tiles; ++tile) {
-    const int row0 = (first * a.tiles + tile) * kRows;
-    if (row0 >= a.L) break;
-    t.turn_to(a, row0 + threadIdx.x / LPR);
-    const bool here = t.live && t.l < a.L;
-    const T *x = static_cast<const T *>(side.x) + t.b * side.sx.b + (here ? t.l * side.sx.l : 0);
-    const T *g = static_cast<const T *>(side.g) + t.b * side.sg.b + (here ? t.l * side.sg.l : 0);
-    T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0);
-    for (int h0 = t.h_lo; h0 < t.h_hi; h0 += kAheadBwd) {
-      uint4 ua[kAheadBwd], ub[kAheadBwd], ga[kAheadBwd], gb[kAheadBwd];
+  for (int e = 0; e < 2; ++e) {
+    const NormSide &side = a.side[e];
+    // this CTA's share [lo, hi) of the side's items; item = (strip * B + b) * chunks + chunk
+    const int64_t all_q = a.items[0], all = all_q + a.items[1];
+    const int64_t from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
+    const int64_t lo = e ? max(from, all_q) - all_q : min(from, all_q), hi = e ? max(to, all_q) - all_q : min(to, all_q);
+    NormLane<T, LPR, IL> t;
+    t.columns(a);
+    float dlo[8], dhi[8];
 #pragma unroll
-      for (int u = 0; u < kAheadBwd; ++u) {
-        ua[u] = ub[u] = ga[u] = gb[u] = make_uint4(0, 0, 0, 0);
-        if (here && h0 + u < t.h_hi) {
-          const T *sx = x + (int64_t)(h0 + u) * side.sx.h, *sg = g + (int64_t)(h0 + u) * side.sg.h;
-          ua[u] = load16(sx + t.off_a);
-          ub[u] = load16(sx + t.off_b);
-          ga[u] = load16(sg + t.off_a);
-          gb[u] = load16(sg + t.off_b);
+    for (int i = 0; i < 8; ++i) dlo[i] = dhi[i] = 0.f;
+    if (lo < hi) {
+      t.e = e;
+      t.weights(a);
+      // where the copies are: an item and a head in it
+      int64_t item = lo;
+      int head = 0, left = 0, row = 0, batch = 0;
+      const T *x = nullptr, *g = nullptr;
+      auto open = [&]() {   // of `item`
+        const int chunk = (int)(item % a.chunks[e]);
+        const int64_t rest = item / a.chunks[e];
+        batch = (int)(rest % a.B), row = (int)(rest / a.B) * kRows + group;
+        head = chunk * a.per_cta[e], left = min(side.heads - head, a.per_cta[e]);
+        const int64_t l = row < a.L ? row : 0;
+        x = static_cast<const T *>(side.x) + batch * side.sx.b + l * side.sx.l + head * side.sx.h;
+        g = static_cast<const T *>(side.g) + batch * side.sg.b + l * side.sg.l + head * side.sg.h;
+      };
+      int stage = 0;
+      auto fetch = [&]() {   // the next head, or nothing behind the last item
+        if (item < hi) {
+          const bool here = t.live && row < a.L;
+          const uint32_t at = slot + stage * (4 * kNormThreads * 16);
+          const T *sx = here ? x : static_cast<const T *>(side.x), *sg = here ? g : static_cast<const T *>(side.g);
+          cp_async16(at, sx + (here ? t.off_a : 0), here);
+          cp_async16(at + kNormThreads * 16, sx + (here ? t.off_b : 0), here);
+          cp_async16(at + 2 * kNormThreads * 16, sg + (here ? t.off_a : 0), here);
+          cp_async16(at + 3 * kNormThreads * 16, sg + (here ? t.off_b : 0), here);
+          x += side.sx.h, g += side.sg.h;
+          if (--left == 0 && ++item < hi) open();
+        }
+        cp_async_commit();
+        stage = stage + 1 == kRing ? 0 : stage + 1;
+      };
+      open();
+      // where the arithmetic is
+      int64_t item_c = lo;
+      int stage_c = 0;
+#pragma unroll 1
+      for (int i = 0; i < kRing - 1; ++i) fetch();
+#pragma unroll 1
+      for (; item_c < hi; ++item_c) {
+        const int chunk = (int)(item_c % a.chunks[e]);
+        const int64_t rest = item_c / a.chunks[e];
+        t.b = (int)(rest % a.B);
+        t.turn_to(a, (int)(rest / a.B) * kRows + group);
+        const int h0 = chunk * a.per_cta[e], count = min(side.heads - h0, a.per_cta[e]);
+        const bool here = t.live && t.l < a.L;
+        T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0) + h0 * side.sy.h;
+#pragma unroll 1
+        for (int h = 0; h < count; ++h) {
+          fetch();
+          cp_async_wait<kRing - 1>();
+          const uint32_t at = slot + stage_c * (4 * kNormThreads * 16);
+          stage_c = stage_c + 1 == kRing ? 0 : stage_c + 1;
+          float va[8], vb[8], xlo[8], xhi[8], glo[8], ghi[8];
+          unpack8<T>(va, lds16(at));
+          unpack8<T>(vb, lds16(at + kNormThreads * 16));
+          to_pairs<IL>(xlo, xhi, va, vb);
+          unpack8<T>(va, lds16(at + 2 * kNormThreads * 16));
+          unpack8<T>(vb, lds16(at + 3 * kNormThreads * 16));
+          to_pairs<IL>(glo, ghi, va, vb);
+          float ss = 0.f, ax = 0.f;
+          float tlo[8], thi[8];   // h x
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ss = fmaf(xlo[i], xlo[i], fmaf(xhi[i], xhi[i], ss));
+            const float hl = glo[i] * t.c[i] + ghi[i] * t.s[i], hh = ghi[i] * t.c[i] - glo[i] * t.s[i];
+            tlo[i] = hl * xlo[i], thi[i] = hh * xhi[i];
+            ax = fmaf(tlo[i], t.wlo[i], fmaf(thi[i], t.whi[i], ax));
+            glo[i] = hl * t.wlo[i], ghi[i] = hh * t.whi[i];
+          }
+          const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, a.eps));
+          const float k = group_sum<LPR>(ax) * inv_d * r * r * r;   // dx = r a - k x (in this order: r^3 may be below fp32's range)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dlo[i] = fmaf(tlo[i], r, dlo[i]);
+            dhi[i] = fmaf(thi[i], r, dhi[i]);
+            glo[i] = fmaf(r, glo[i], -k * xlo[i]);
+            ghi[i] = fmaf(r, ghi[i], -k * xhi[i]);
+          }
+          from_pairs<IL>(va, vb, glo, ghi);
+          if (here) {
+            *reinterpret_cast<uint4 *>(y + t.off_a) = pack8<T>(va);
+            *reinterpret_cast<uint4 *>(y + t.off_b) = pack8<T>(vb);
+          }
+          y += side.sy.h;
         }
       }
+      cp_async_wait<0>();
+    }
+    if (!partial) continue;
+    // groups of a warp, then warps, then one row
+    float va[8], vb[8];
+    from_pairs<IL>(va, vb, dlo, dhi);
 #pragma unroll
-      for (int u = 0; u < kAheadBwd; ++u) {
-        if (h0 + u >= t.h_hi) break;
-        float va[8], vb[8], xlo[8], xhi[8], glo[8], ghi[8];
-        unpack8<T>(va, ua[u]);
-        unpack8<T>(vb, ub[u]);
-        to_pairs<IL>(xlo, xhi, va, vb);
-        unpack8<T>(va, ga[u]);
-        unpack8<T>(vb, gb[u]);
-        to_pairs<IL>(glo, ghi, va, vb);
-        float ss = 0.f, ax = 0.f;
+    for (int m = LPR; m < 32; m *= 2)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss = fmaf(xlo[i], xlo[i], fmaf(xhi[i], xhi[i], ss));
-          const float hl = glo[i] * t.c[i] + ghi[i] * t.s[i], hh = ghi[i] * t.c[i] - glo[i] * t.s[i];
-          glo[i] = hl, ghi[i] = hh;
-          ax = fmaf(hl * t.wlo[i], xlo[i], fmaf(hh * t.whi[i], xhi[i], ax));
-        }
-        const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, a.eps));
-        const float k = group_sum<LPR>(ax) * inv_d * r * r;   // dx = r (a - k x)
+      for (int i = 0; i < 8; ++i) {
+        va[i] += __shfl_xor_sync(0xffffffffu, va[i], m);
+        vb[i] += __shfl_xor_sync(0xffffffffu, vb[i], m);
+      }
+    __syncthreads();   // every thread is through with the ring
+    if ((threadIdx.x & 31) < LPR && t.live) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dlo[i] = fmaf(glo[i], xlo[i] * r, dlo[i]);
-          dhi[i] = fmaf(ghi[i], xhi[i] * r, dhi[i]);
-          glo[i] = r * (glo[i] * t.wlo[i] - k * xlo[i]);
-          ghi[i] = r * (ghi[i] * t.whi[i] - k * xhi[i]);
-        }
-        from_pairs<IL>(va, vb, glo, ghi);
-        if (here) {
-          T *dst = y + (int64_t)(h0 + u) * side.sy.h;
-          *reinterpret_cast<uint4 *>(dst + t.off_a) = pack8<T>(va);
-          *reinterpret_cast<uint4 *>(dst + t.off_b) = pack8<T>(vb);
-        }
+      for (int i = 0; i < 8; ++i) {
+        sums[threadIdx.x / 32][t.off_a + i] = va[i];
+        sums[threadIdx.x / 32][t.off_b + i] = vb[i];
       }
     }
-  }
-
-  if (!partial) return;
-  // groups of a warp, then warps, then one row
-  float va[8], vb[8];
-  from_pairs<IL>(va, vb, dlo, dhi);
+    __syncthreads();
+    float *out = partial + ((int64_t)e * gridDim.x + blockIdx.x) * a.D;
+    for (int d = threadIdx.x; d < a.D; d += kNormThreads) {
+      float v = 0.f;
 #pragma unroll
-  for (int m = LPR; m < 32; m *= 2)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      va[i] += __shfl_xor_sync(0xffffffffu, va[i], m);
-      vb[i] += __shfl_xor_sync(0xffffffffu, vb[i], m);
+      for (int w = 0; w < kWarps; ++w) v += sums[w][d];
+      out[d] = v;
     }
-  if ((threadIdx.x & 31) < LPR && t.live) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sums[threadIdx.x / 32][t.off_a + i] = va[i];
-      sums[threadIdx.x / 32][t.off_b + i] = vb[i];
-    }
-  }
-  __syncthreads();
-  // this CTA's row among those of its side: CTAs of a side in order
-  const int z = (int)(blockIdx.x % Z) - (t.e ? a.chunks[0] : 0);
-  const int64_t rest = blockIdx.x / Z, sides = gridDim.x / Z;
-  const int64_t row = (t.e ? sides * a.chunks[0] : 0) + rest * a.chunks[t.e] + z;
-  for (int d = threadIdx.x; d < a.D; d += kNormThreads) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += sums[w][d];
-    partial[row * a.D + d] = v;
+    __syncthreads();   // before the next side's copies
   }
 }
 
 // dw from the partial rows: a CTA has 8 columns of one side, 128 threads a column, and adds them in a fixed order.
 struct WeightGrad {
   void *out[2];
-  int rows[2];
+  int rows;
 };
 template <typename T>
 __global__ void __launch_bounds__(1024) weight_grad_kernel(const float *partial, WeightGrad w, int D, int f32) {
   __shared__ float sums[128][9];
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int e = blockIdx.y, col = blockIdx.x * 8 + threadIdx.x % 8, lane = threadIdx.x / 8;
-  const float *p = partial + (e ? (int64_t)w.rows[0] * D : 0) + col;
+  const float *p = partial + (int64_t)e * w.rows * D + col;
   float v = 0.f;
 #pragma unroll 8
-  for (int i = lane; i < w.rows[e]; i += 128) v += p[(int64_t)i * D];
+  for (int i = lane; i < w.rows; i += 128) v += p[(int64_t)i * D];
   sums[lane][threadIdx.x % 8] = v;
   __syncthreads();
   for (int n = 64; n >= 1; n /= 2) {
@@ -315,28 +369,31 @@ int check_norm(const fa_norm_rotary_args *a) {
   return FA_OK;
 }
 
-// A CTA's heads: all that share a position's angles, but fewer where the grid would not be `waves` of 4 CTAs an SM.
-// (`tiles`: positions groups a CTA walks on top, where it would be deeper; for the backward, whose CTAs leave a row of
-// partial sums each.)
-int64_t plan_norm(const fa_norm_rotary_args *s, NormArgs *a, int waves, bool walk) {
+int sms() {
+  const int n = sm_count_of_device();
+  return n ? n : 148;   // (sizes asked for without a GPU)
+}
+
+// Heads that a thread walks with a position's angles and the weights in its registers: as many as leave the grid `waves` of
+// `resident` CTAs an SM deep, `most` at most.  Forward, B=2 H=48+8 L=16384 D=128: 163 us with up to 16 heads, 170 with up
+// to 8; B=3 H=20+4 L=1999 D=64: 12 us by this rule, 15 with grids 8 waves deep, whose threads load angles and weights for
+// each head.  Returns the number of (strip of positions, chunk of heads).
+int64_t plan_norm(const fa_norm_rotary_args *s, NormArgs *a, int resident, int waves, int most) {
   const int rows = kNormThreads / lanes_per_row(s->D);
-  const int64_t positions = (int64_t)((s->L + rows - 1) / rows) * s->B, want = (int64_t)148 * 4 * waves;
+  const int64_t positions = (int64_t)((s->L + rows - 1) / rows) * s->B, want = (int64_t)sms() * resident * waves;
   const int all = s->H + s->Hk;
   int per = 1;
-  while (per < all && positions * ((all + 2 * per - 1) / (2 * per)) >= want) per *= 2;
-  per = per > 8 ? 8 : per;
+  while (per < most && positions * ((all + 2 * per - 1) / (2 * per)) >= want) per *= 2;
   for (int e = 0; e < 2; ++e) {
     const int heads = e ? s->Hk : s->H;
-    a->per_cta[e] = per < heads ? per : heads;
+    a->per_cta[e] = std::min(per, heads);
     a->chunks[e] = (heads + a->per_cta[e] - 1) / a->per_cta[e];
+    a->items[e] = positions * a->chunks[e];
   }
-  const int Z = a->chunks[0] + a->chunks[1];
-  int tiles = 1;
-  const int64_t strips = (s->L + rows - 1) / rows;
-  while (walk && strips > tiles && (strips + 2 * tiles - 1) / (2 * tiles) * s->B * Z >= want) tiles *= 2;
-  a->tiles = tiles;
-  return (strips + tiles - 1) / tiles * s->B * Z;
+  return a->items[0] + a->items[1];
 }
+// CTAs of the backward: all that are resident at once, each with a share of the items
+int64_t backward_ctas(int64_t items) { return std::min(items, (int64_t)sms() * kBackwardCtas); }
 
 void fill_norm(const fa_norm_rotary_args *s, NormArgs *a) {
   a->cos = s->cos, a->sin = s->sin, a->positions = s->positions, a->pos_stride_b = s->pos_stride_b, a->eps = s->eps;
@@ -345,8 +402,6 @@ void fill_norm(const fa_norm_rotary_args *s, NormArgs *a) {
   a->side[0].weight = s->q_weight, a->side[1].weight = s->k_weight;
   a->side[0].heads = s->H, a->side[1].heads = s->Hk;
 }
-
-constexpr int kForwardWaves = 16, kBackwardWaves = 4;
 
 template <typename T, int LPR, bool IL>
 int launch_norm(const NormArgs &a, int64_t grid, bool backward, float *partial, cudaStream_t s) {
@@ -393,13 +448,13 @@ extern "C" int fa_qk_norm_rotary_fwd(const fa_norm_rotary_args *p, const fa_tens
   fill_norm(p, &a);
   a.side[0].x = q->ptr, a.side[0].sx = strides_of(q), a.side[0].y = q_out->ptr, a.side[0].sy = strides_of(q_out);
   a.side[1].x = k->ptr, a.side[1].sx = strides_of(k), a.side[1].y = k_out->ptr, a.side[1].sy = strides_of(k_out);
-  return dispatch_norm(p, a, plan_norm(p, &a, kForwardWaves, false), false, nullptr, static_cast<cudaStream_t>(stream));
+  return dispatch_norm(p, a, plan_norm(p, &a, kForwardCtas, 1, 16), false, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t fa_qk_norm_rotary_bwd_workspace_bytes(const fa_norm_rotary_args *p) {
   if (check_norm(p) || p->B == 0 || p->L == 0) return 0;
   NormArgs a{};
-  return plan_norm(p, &a, kBackwardWaves, true) * p->D * 4;
+  return 2 * backward_ctas(plan_norm(p, &a, kBackwardCtas, 4, 8)) * p->D * 4;
 }
 
 extern "C" int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *p, const fa_tensor4 *q, const fa_tensor4 *k,
@@ -427,13 +482,12 @@ extern "C" int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *p, const fa_tens
     a.side[e].g = gs[e]->ptr, a.side[e].sg = strides_of(gs[e]);
     a.side[e].y = ds[e]->ptr, a.side[e].sy = strides_of(ds[e]);
   }
-  const int64_t grid = plan_norm(p, &a, kBackwardWaves, true);
-  if (weights && (!workspace || !aligned16(workspace) || workspace_bytes < grid * p->D * 4)) return FA_ERR_WORKSPACE;
+  const int64_t grid = backward_ctas(plan_norm(p, &a, kBackwardCtas, 4, 8));
+  if (weights && (!workspace || !aligned16(workspace) || workspace_bytes < 2 * grid * p->D * 4)) return FA_ERR_WORKSPACE;
   float *partial = weights ? static_cast<float *>(workspace) : nullptr;
   if (int st = dispatch_norm(p, a, grid, true, partial, s)) return st;
   if (!weights) return FA_OK;
-  const int64_t strips = grid / (a.chunks[0] + a.chunks[1]);
-  const WeightGrad w{{dq_weight, dk_weight}, {(int)(strips * a.chunks[0]), (int)(strips * a.chunks[1])}};
+  const WeightGrad w{{dq_weight, dk_weight}, (int)grid};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;

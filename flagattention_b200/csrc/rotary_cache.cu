@@ -10,9 +10,11 @@
 // Scales are powers of two, the least that holds the block.  That costs a floating code nothing (e4m3 has the same
 // relative step at every exponent), and when a later token needs a larger one the old codes only move in exponent: exact
 // but below 2^-6 of the new scale, where e4m3 loses bits.  A block filled token by token is the block filled at once.
-// An e4m3 code jumps at its borders, so a key is worked out in 64 bits and taken to fp32 by rounding to odd (truncate, and
-// set the last bit if anything was lost): that keeps every comparison and the second rounding right.  The 64-bit
-// units do it beside the stream: three operations an element of k, a tenth of the elements of a grouped-query layer.
+// An e4m3 code jumps at its borders, and so does a scale: a key is worked out in 64 bits and taken to fp32 by rounding to odd
+// (truncated, the last bit set if anything was lost), which keeps comparisons and the second rounding right.  (fp32 with a
+// known error and 64 bits only where that leaves two codes: slower, 7.3 us for 4.5 at 64 single tokens, 53 for 44 at 5800
+// rows of prompts.  Some warp always has such an element, and the second way costs the first one its registers.)
+
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -26,14 +28,17 @@ namespace fa {
 
 constexpr int kCacheThreads = 128;
 constexpr int kTile = 32;     // rows whose units a CTA of the 8-bit part finds at once, one a lane
-constexpr int kPasses = 4;    // 16-byte pieces of a thread that stay in registers between the maximum and the codes
+constexpr int kAhead = 4;     // heads of a row whose loads are in flight
 
 struct RotaryCache {
   fa_rotary_cache_args p;
-  int unit_ctas;    // CTAs of the unit part, in front: a unit takes longer than a row
+  int unit_ctas;    // CTAs of the unit part, in front
   int per_cta;      // heads one of them walks
-  int chunks;       // CTAs that share a group of tokens
-  int unit_ctas_y;  // 8 bits: CTAs that share a tile of rows
+  int chunks;       // CTAs that share a group of tokens, and how many of them have heads of q, of k and of v
+  int chunks_of[3];
+  int unit_ctas_y;  // CTAs that share a tile of rows
+  int unit_heads;   // heads of a block that a CTA takes in turn, and how many CTAs that is for k or v
+  int unit_chunks;
 };
 
 __device__ __forceinline__ uint4 read16(const void *p) { return *reinterpret_cast<const uint4 *>(p); }
@@ -133,78 +138,106 @@ __device__ __forceinline__ void row_part(const RotaryCache &a) {
   constexpr int kRows = kCacheThreads / LPR;
   const Lane<LPR, IL> lane(p.rotary_dim);
   const unsigned cta = blockIdx.x - a.unit_ctas;
-  const int z = cta % a.chunks, row = (int)(cta / a.chunks) * kRows + (int)threadIdx.x / LPR;
-  const Token t = find_token(p, row);
+  int z = cta % a.chunks;
+  const int row = (int)(cta / a.chunks) * kRows + (int)threadIdx.x / LPR;
   const bool here = row < p.num_tokens;
-  const int heads = p.num_q_heads + (p.key_scales ? 0 : 2 * p.num_kv_heads);
-  const int h_lo = z * a.per_cta, h_hi = min(heads, h_lo + a.per_cta);
-  const int v_lo = p.num_q_heads + p.num_kv_heads;   // heads from here on are values
-  int64_t blk = -1;
-  if (h_hi > p.num_q_heads && t.valid) blk = block_of(p, t.seq, t.place / p.block_size);
-  const int64_t slot = blk * p.kv_stride_b + (int64_t)(t.place % p.block_size) * p.kv_stride_t;
-  float c[8], s[8], wlo[8], whi[8];
-  if (h_lo < v_lo) lane.angles(p, t.valid ? table_row(p, row, t.place) : 0, t.valid, c, s);
-  const bool norm = p.q_weight != nullptr;
-  const float inv_d = 1.f / p.head_size;
-  int have = -1;   // whose weights are in the registers: 0 q, 1 k
-
-  for (int h0 = h_lo; h0 < h_hi; h0 += kPasses) {
-    uint4 ua[kPasses], ub[kPasses];
+  // a CTA has heads of q, of k or of v
+  int kind = 0;
+  if (z >= a.chunks_of[0]) z -= a.chunks_of[0], kind = 1;
+  if (kind && z >= a.chunks_of[1]) z -= a.chunks_of[1], kind = 2;
+  const int heads = kind ? p.num_kv_heads : p.num_q_heads;
+  const int h_lo = z * a.per_cta, count = min(heads - h_lo, a.per_cta);
+  const int64_t src_h = kind == 0 ? p.q_stride_h : kind == 1 ? p.k_stride_h : p.v_stride_h;
+  const T *src = static_cast<const T *>(kind == 0 ? p.query : kind == 1 ? p.key : p.value) +
+                 row * (kind == 0 ? p.q_stride_t : kind == 1 ? p.k_stride_t : p.v_stride_t) + h_lo * src_h;
+  uint4 ua[kAhead], ub[kAhead];
+  auto load = [&](int left) {
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      const int h = h0 + u;
+    for (int u = 0; u < kAhead; ++u) {
       ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
-      if (!here || h >= h_hi || !t.valid) continue;
-      const T *src = h < p.num_q_heads ? static_cast<const T *>(p.query) + row * p.q_stride_t + h * p.q_stride_h
-                     : h < v_lo ? static_cast<const T *>(p.key) + row * p.k_stride_t + (h - p.num_q_heads) * p.k_stride_h
-                                : static_cast<const T *>(p.value) + row * p.v_stride_t + (h - v_lo) * p.v_stride_h;
-      ua[u] = read16(src + lane.off_a);
-      ub[u] = read16(src + lane.off_b);
+      if (here && u < left) {
+        ua[u] = read16(src + lane.off_a);
+        ub[u] = read16(src + lane.off_b);
+      }
+      src += src_h;
     }
-#pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      const int h = h0 + u;
-      if (h >= h_hi) break;   // (as in all comparisons of h: the same for the whole CTA)
-      if (h < v_lo) {
-        float va[8], vb[8], lo[8], hi[8], ylo[8], yhi[8];
-        unpack8<T>(va, ua[u]);
-        unpack8<T>(vb, ub[u]);
-        to_pairs<IL>(lo, hi, va, vb);
-        if (norm) {
-          const int e = h >= p.num_q_heads;
-          if (have != e) lane.template weights<T>(p, e ? p.k_weight : p.q_weight, wlo, whi);
-          have = e;
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(va[i], va[i], fmaf(vb[i], vb[i], ss));
-          const float r = rsqrtf(fmaf(lanes_sum<LPR>(ss), inv_d, p.eps));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) lo[i] *= r * wlo[i], hi[i] *= r * whi[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ylo[i] = lo[i] * c[i] - hi[i] * s[i];
-          yhi[i] = hi[i] * c[i] + lo[i] * s[i];
-        }
-        from_pairs<IL>(va, vb, ylo, yhi);
-        if (t.valid) ua[u] = pack8<T>(va), ub[u] = pack8<T>(vb);   // (a row without a place stays 0)
-      }
-      T *dst;
-      if (h < p.num_q_heads) {
-        if (!here) continue;
-        dst = static_cast<T *>(p.out) + row * p.o_stride_t + h * p.o_stride_h;
-      } else {
-        if (blk < 0) continue;
-        dst = h < v_lo ? static_cast<T *>(p.key_cache) + slot + (h - p.num_q_heads) * p.kv_stride_h
-                       : static_cast<T *>(p.value_cache) + slot + (h - v_lo) * p.kv_stride_h;
-      }
+  };
+  load(count);   // in flight while the rows' places are found
+  const Token t = find_token(p, row);
+  T *dst;
+  int64_t dst_h = kind ? p.kv_stride_h : p.o_stride_h;
+  bool writes = here;
+  if (kind) {
+    const int64_t blk = t.valid ? block_of(p, t.seq, t.place / p.block_size) : -1;
+    writes = blk >= 0;
+    dst = static_cast<T *>(kind == 1 ? p.key_cache : p.value_cache) + max(blk, (int64_t)0) * p.kv_stride_b +
+          (int64_t)(t.place % p.block_size) * p.kv_stride_t;
+  } else {
+    dst = static_cast<T *>(p.out) + row * p.o_stride_t;
+  }
+  dst += h_lo * dst_h;
+  auto store = [&](int u) {
+    if (writes) {
       *reinterpret_cast<uint4 *>(dst + lane.off_a) = ua[u];
       *reinterpret_cast<uint4 *>(dst + lane.off_b) = ub[u];
     }
+    dst += dst_h;
+  };
+  if (kind == 2) {
+    for (int left = count;;) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u < left) store(u);
+      if ((left -= kAhead) <= 0) return;
+      load(left);
+    }
+  }
+  // the rotation and the weights in one: y_lo = r (x_lo ll - x_hi lh), y_hi = r (x_hi hh + x_lo hl)
+  float ll[8], lh[8], hh[8], hl[8];
+  lane.angles(p, t.valid ? table_row(p, row, t.place) : 0, t.valid, ll, lh);
+  const bool norm = p.q_weight != nullptr;
+  {
+    float wlo[8], whi[8];
+    if (norm) lane.template weights<T>(p, kind ? p.k_weight : p.q_weight, wlo, whi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = ll[i], s = lh[i], l = norm ? wlo[i] : 1.f, h = norm ? whi[i] : 1.f;
+      ll[i] = c * l, hh[i] = c * h, lh[i] = s * h, hl[i] = s * l;
+    }
+  }
+  const float inv_d = 1.f / p.head_size;
+  for (int left = count;;) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (u >= left) break;   // the same for the whole CTA
+      float va[8], vb[8], lo[8], hi[8], ylo[8], yhi[8];
+      unpack8<T>(va, ua[u]);
+      unpack8<T>(vb, ub[u]);
+      float r = 1.f;
+      if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(va[i], va[i], fmaf(vb[i], vb[i], ss));
+        r = rsqrtf(fmaf(lanes_sum<LPR>(ss), inv_d, p.eps));
+      }
+      to_pairs<IL>(lo, hi, va, vb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ylo[i] = (lo[i] * ll[i] - hi[i] * lh[i]) * r;
+        yhi[i] = (hi[i] * hh[i] + lo[i] * hl[i]) * r;
+      }
+      from_pairs<IL>(va, vb, ylo, yhi);
+      ua[u] = pack8<T>(va), ub[u] = pack8<T>(vb);
+      if (!t.valid) ua[u] = ub[u] = make_uint4(0, 0, 0, 0);   // (whatever the row holds)
+      store(u);
+    }
+    if ((left -= kAhead) <= 0) return;
+    load(left);
   }
 }
 
-// ---- units of an 8-bit cache: the new tokens of one block and kv head, of k or of v, one warp ------------------------------
+// ---- units of an 8-bit cache: the new tokens of one block and kv head, of k or of v --------------------------------------
+// Taken by a CTA, a row of a pass to each group of lanes; or by a warp where every unit is one token.
 // fp32 by rounding to odd: between the 64-bit value and any number of fewer bits it compares as the value does, and
 // rounds to where the value would
 __device__ __forceinline__ float to_odd(double v) {
@@ -228,101 +261,98 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
-template <typename T, int LPR, bool IL>
+// The threads that work on a unit, TEAM of them, and the row of a pass that each has a part of.
+template <typename T, int LPR, bool IL, int TEAM>
 struct Unit {
-  static constexpr int kRowsPass = 32 / LPR;
-  static constexpr int kRowsChunk = kRowsPass * kPasses;
+  static constexpr int kRowsPass = TEAM / LPR;
   const fa_rotary_cache_args &p;
   const Lane<LPR, IL> &lane;
-  const T *src;        // the head's row of the first token
-  int64_t src_stride;
   int row0, place0, n;   // first token: its row and place; tokens of the unit
   bool key;
 
-  // fp32 values of this thread's elements of the rows chunk * kRowsChunk + pass * kRowsPass + lane / LPR
-  __device__ __forceinline__ void values(int chunk, float (&v)[kPasses][16]) const {
-    uint4 ua[kPasses], ub[kPasses];
-#pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      const int i = chunk * kRowsChunk + u * kRowsPass + (int)(threadIdx.x & 31) / LPR;
-      ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
-      if (i < n) {
-        ua[u] = read16(src + i * src_stride + lane.off_a);
-        ub[u] = read16(src + i * src_stride + lane.off_b);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      if (chunk * kRowsChunk + u * kRowsPass >= n) break;   // the same for the whole warp
-      const int i = chunk * kRowsChunk + u * kRowsPass + (int)(threadIdx.x & 31) / LPR;
-      float va[8], vb[8];
-      unpack8<T>(va, ua[u]);
-      unpack8<T>(vb, ub[u]);
-      if (key) {
-        float c[8], s[8], lo[8], hi[8], wlo[8], whi[8];
-        lane.angles(p, i < n ? table_row(p, row0 + i, place0 + i) : 0, i < n, c, s);
-        double r = 1.0;
-        if (p.k_weight) {
-          double ss = 0.0;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) ss += (double)va[k] * va[k] + (double)vb[k] * vb[k];
-          r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + (double)p.eps);
-          lane.template weights<T>(p, p.k_weight, wlo, whi);
-        }
-        to_pairs<IL>(lo, hi, va, vb);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          double l = lo[k], h = hi[k];
-          if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
-          lo[k] = to_odd(l * c[k] - h * s[k]);
-          hi[k] = to_odd(h * c[k] + l * s[k]);
-        }
-        from_pairs<IL>(va, vb, lo, hi);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[u][k] = va[k], v[u][8 + k] = vb[k];
+  static __device__ __forceinline__ int thread() { return threadIdx.x % TEAM; }
+  static __device__ __forceinline__ int row_of(int pass) { return pass * kRowsPass + thread() / LPR; }
+
+  __device__ __forceinline__ void load(int pass, int head, uint4 (&u)[2]) const {
+    const int i = row_of(pass);
+    u[0] = u[1] = make_uint4(0, 0, 0, 0);
+    if (i < n) {
+      const T *src = key ? static_cast<const T *>(p.key) + (row0 + i) * p.k_stride_t + head * p.k_stride_h
+                         : static_cast<const T *>(p.value) + (row0 + i) * p.v_stride_t + head * p.v_stride_h;
+      u[0] = read16(src + lane.off_a);
+      u[1] = read16(src + lane.off_b);
     }
   }
-  __device__ __forceinline__ uint32_t largest(int chunk, const float (&v)[kPasses][16]) const {
+  __device__ __forceinline__ void angles(int pass, float (&c)[8], float (&s)[8]) const {
+    const int i = row_of(pass);
+    if (key) lane.angles(p, i < n ? table_row(p, row0 + i, place0 + i) : 0, i < n, c, s);
+  }
+  // fp32 values of what load() brought, of a key from 64 bits
+  __device__ __forceinline__ void values(const uint4 (&u)[2], const float (&c)[8], const float (&s)[8], float (&lo)[8],
+                                         float (&hi)[8]) const {
+    float va[8], vb[8];
+    unpack8<T>(va, u[0]);
+    unpack8<T>(vb, u[1]);
+    to_pairs<IL>(lo, hi, va, vb);
+    if (!key) return;
+    float wlo[8], whi[8];
+    double r = 1.0;
+    if (p.k_weight) {
+      double ss = 0.0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss += (double)va[k] * va[k] + (double)vb[k] * vb[k];
+      r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + (double)p.eps);
+      lane.template weights<T>(p, p.k_weight, wlo, whi);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      double l = lo[k], h = hi[k];
+      if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
+      lo[k] = to_odd(l * c[k] - h * s[k]);
+      hi[k] = to_odd(h * c[k] + l * s[k]);
+    }
+  }
+  __device__ __forceinline__ uint32_t largest(int pass, const float (&lo)[8], const float (&hi)[8]) const {
     uint32_t most = 0;
+    if (row_of(pass) < n) {
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      if (chunk * kRowsChunk + u * kRowsPass >= n) break;
-      if (chunk * kRowsChunk + u * kRowsPass + (int)(threadIdx.x & 31) / LPR < n) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint32_t bits = __float_as_uint(v[u][k]) & 0x7fffffffu;
-          most = max(most, bits < 0x7f800000u ? bits : 0u);   // an infinity saturates, a NaN stays one: no scale holds them
-        }
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t x = __float_as_uint(lo[k]) & 0x7fffffffu, y = __float_as_uint(hi[k]) & 0x7fffffffu;
+        most = max(most, x < 0x7f800000u ? x : 0u);   // an infinity saturates, a NaN stays one: no scale holds them
+        most = max(most, y < 0x7f800000u ? y : 0u);
       }
     }
     return most;
   }
-  __device__ __forceinline__ void store(int chunk, const float (&v)[kPasses][16], float scale, uint8_t *dst) const {
-    const double inv = 1.0 / (double)scale;
-    const float inv_f = (float)inv;
-    const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0;   // as this kernel leaves them: the product is exact
+  __device__ __forceinline__ void store(int pass, const float (&lo)[8], const float (&hi)[8], float scale,
+                                        uint8_t *dst) const {
+    const int i = row_of(pass);
+    if (i >= n) return;
+    float x[8], y[8], a[8], b[8];
+    if ((__float_as_uint(scale) & 0x7fffffu) == 0) {   // a power of two, as this kernel leaves them: products are exact
+      const float inv = 1.f / scale;
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      if (chunk * kRowsChunk + u * kRowsPass >= n) break;
-      const int i = chunk * kRowsChunk + u * kRowsPass + (int)(threadIdx.x & 31) / LPR;
-      if (i >= n) continue;
-      float q[16];
+      for (int k = 0; k < 8; ++k) x[k] = lo[k] * inv, y[k] = hi[k] * inv;
+    } else {
+      const double inv = 1.0 / (double)scale;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) q[k] = power ? v[u][k] * inv_f : to_odd((double)v[u][k] * inv);
-      uint8_t *at = dst + i * p.kv_stride_t;
-      *reinterpret_cast<uint2 *>(at + lane.off_a) =
-          make_uint2(pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7]));
-      *reinterpret_cast<uint2 *>(at + lane.off_b) =
-          make_uint2(pack_e4m3(q[8], q[9], q[10], q[11]), pack_e4m3(q[12], q[13], q[14], q[15]));
+      for (int k = 0; k < 8; ++k) x[k] = to_odd((double)lo[k] * inv), y[k] = to_odd((double)hi[k] * inv);
     }
+    from_pairs<IL>(a, b, x, y);
+    uint8_t *at = dst + i * p.kv_stride_t;
+    *reinterpret_cast<uint2 *>(at + lane.off_a) =
+        make_uint2(pack_e4m3(a[0], a[1], a[2], a[3]), pack_e4m3(a[4], a[5], a[6], a[7]));
+    *reinterpret_cast<uint2 *>(at + lane.off_b) =
+        make_uint2(pack_e4m3(b[0], b[1], b[2], b[3]), pack_e4m3(b[4], b[5], b[6], b[7]));
   }
 };
 
-// codes of `rows` rows by `ratio` < 1
-__device__ __forceinline__ void move_codes(uint8_t *dst, int64_t stride, int rows, int head_size, double ratio) {
+// codes of `rows` rows by `ratio` < 1, `threads` threads of which this is the `thread`-th
+__device__ __forceinline__ void move_codes(uint8_t *dst, int64_t stride, int rows, int head_size, double ratio, int thread,
+                                           int threads) {
   const int per_row = head_size / 16;
-  for (int i = threadIdx.x & 31; i < rows * per_row; i += 32) {
+#pragma unroll 1
+  for (int i = thread; i < rows * per_row; i += threads) {
     uint4 *at = reinterpret_cast<uint4 *>(dst + (i / per_row) * stride + i % per_row * 16);
     const uint4 u = *at;
     uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -335,59 +365,103 @@ __device__ __forceinline__ void move_codes(uint8_t *dst, int64_t stride, int row
   }
 }
 
-template <typename T, int LPR, bool IL>
-__device__ __forceinline__ void unit(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq, int place,
-                                     int left, int head, bool key) {
-  const int64_t blk = block_of(p, seq, place / p.block_size);
-  if (blk < 0) return;
+// The units of a block's heads [h_lo, h_hi), one after another: the next head's loads are in flight, and the rows' angles
+// stay in registers.
+template <typename T, int LPR, bool IL, int TEAM>
+__device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq, int place,
+                                         int left, int h_lo, int h_hi, bool key, uint32_t *shared_most) {
+  constexpr int kWarps = TEAM / 32;
   const int off = place % p.block_size;
-  const T *src = key ? static_cast<const T *>(p.key) + row * p.k_stride_t + head * p.k_stride_h
-                     : static_cast<const T *>(p.value) + row * p.v_stride_t + head * p.v_stride_h;
-  const Unit<T, LPR, IL> u{p, lane, src, key ? p.k_stride_t : p.v_stride_t, row, place, min(left, p.block_size - off), key};
-  float *scale = (key ? p.key_scales : p.value_scales) + blk * p.num_kv_heads + head;
-  uint8_t *cache = static_cast<uint8_t *>(key ? p.key_cache : p.value_cache) + blk * p.kv_stride_b + head * p.kv_stride_h;
-  const float old = off ? *scale : 0.f;   // a block's first token: what the block held before is over
-  const int chunks = (u.n + u.kRowsChunk - 1) / u.kRowsChunk;
-  float v[kPasses][16];
-  uint32_t most = 0;
-  for (int i = 0; i < chunks; ++i) {
-    u.values(i, v);
-    most = max(most, u.largest(i, v));
+  const Unit<T, LPR, IL, TEAM> u{p, lane, row, place, min(left, p.block_size - off), key};
+  const int passes = (u.n + u.kRowsPass - 1) / u.kRowsPass;
+  uint4 x[2];
+  float c[8], s[8], lo[8], hi[8];
+  u.load(0, h_lo, x);
+  u.angles(0, c, s);
+  const int64_t blk = block_of(p, seq, place / p.block_size);
+  if (blk < 0) return;   // (the same for the whole team)
+  float *scales = (key ? p.key_scales : p.value_scales) + blk * p.num_kv_heads;
+  uint8_t *caches = static_cast<uint8_t *>(key ? p.key_cache : p.value_cache) + blk * p.kv_stride_b;
+#pragma unroll 1
+  for (int h = h_lo; h < h_hi; ++h) {
+    const float old = off ? scales[h] : 0.f;   // a block's first token: what the block held before is over
+    uint8_t *cache = caches + h * p.kv_stride_h, *dst = cache + off * p.kv_stride_t;
+    // The values' maximum, in one step for each pass; then their codes, from what one pass left in the registers, or by
+    // the same steps once more.
+    const int steps = passes == 1 ? 1 : 2 * passes;
+    uint32_t most = 0;
+    float now = 0.f;
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const int pass = step < passes ? step : step - passes;
+      if (passes > 1) u.angles(pass, c, s);
+      u.values(x, c, s, lo, hi);
+      if (step + 1 < steps) u.load(pass + 1 < passes ? pass + 1 : 0, h, x);
+      else if (h + 1 < h_hi) u.load(0, h + 1, x);
+      if (step < passes) most = max(most, u.largest(pass, lo, hi));
+      if (step == passes - 1) {
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (kWarps > 1) {   // the team's
+          uint32_t *shared = shared_most + (h & 1) * kWarps;   // (no warp is a whole head ahead of another)
+          if ((threadIdx.x & 31) == 0) shared[threadIdx.x / 32] = most;
+          __syncthreads();   // (and every thread has its old scale)
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) most = max(most, shared[w]);
+        }
+        now = scale_for(most);
+        now = fmaxf(old, now);
+        if (off && now > old)
+          move_codes(cache, p.kv_stride_t, off, p.head_size, (double)old / (double)now, u.thread(), TEAM);
+      }
+      if (passes == 1 || step >= passes)
+        u.store(pass, lo, hi, now, dst);
+    }
+    if (u.thread() == 0) scales[h] = now;
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  const float now = fmaxf(old, scale_for(most));
-  if (off && now > old) move_codes(cache, p.kv_stride_t, off, p.head_size, (double)old / (double)now);
-  uint8_t *dst = cache + off * p.kv_stride_t;
-  for (int i = 0; i < chunks; ++i) {
-    if (chunks > 1) u.values(i, v);   // what one chunk holds stays in the registers
-    u.store(i, v, now, dst);
-  }
-  if ((threadIdx.x & 31) == 0) *scale = now;
 }
 
-template <typename T, int LPR, bool IL>
+template <typename T, int LPR, bool IL, bool ONE>
 __device__ __forceinline__ void unit_part(const RotaryCache &a) {
   const fa_rotary_cache_args &p = a.p;
   const Lane<LPR, IL> lane(p.rotary_dim);
-  const int cta = blockIdx.x, warp = threadIdx.x / 32;
-  const int tile = cta / a.unit_ctas_y, stride = a.unit_ctas_y * (kCacheThreads / 32);
-  const int lane_id = threadIdx.x & 31;
-  // (one token a sequence: every row is a unit, and a tile has as many as it has rows)
+  const int per_row = 2 * p.num_kv_heads, warp = threadIdx.x / 32, lane_id = threadIdx.x & 31;
+  if (ONE) {
+    const int64_t i = (int64_t)blockIdx.x * (kCacheThreads / 32) + warp;
+    const int row = (int)(i / per_row), rest = (int)(i % per_row);
+    if (row >= p.num_tokens) return;
+    const Token t = find_token(p, row);
+    if (t.valid)
+      units_of<T, LPR, IL, 32>(p, lane, row, t.seq, t.place, 1, rest / 2, rest / 2 + 1, rest % 2 == 0, nullptr);
+    return;
+  }
+  __shared__ uint32_t shared_most[2 * kCacheThreads / 32];
+  const int tile = blockIdx.x / a.unit_ctas_y, y = blockIdx.x % a.unit_ctas_y;
   const Token t = find_token(p, tile * kTile + lane_id);
   const bool leads = t.valid && (t.first || t.place == 0 || t.place % p.block_size == 0);
-  const unsigned leaders = __ballot_sync(0xffffffffu, leads);
-  const int units = __popc(leaders) * p.num_kv_heads * 2;
-  for (int i = cta % a.unit_ctas_y * (kCacheThreads / 32) + warp; i < units; i += stride) {
-    const int from = __fns(leaders, 0, i / (2 * p.num_kv_heads) + 1), rest = i % (2 * p.num_kv_heads);
-    unit<T, LPR, IL>(p, lane, tile * kTile + from, __shfl_sync(0xffffffffu, t.seq, from),
-                     __shfl_sync(0xffffffffu, t.place, from), __shfl_sync(0xffffffffu, t.left, from), rest / 2,
-                     rest % 2 == 0);
+  const unsigned several = __ballot_sync(0xffffffffu, leads && t.left > 1), single = __ballot_sync(0xffffffffu, leads && t.left == 1);
+  auto from_lane = [&](int x, int from) { return __shfl_sync(0xffffffffu, x, from); };
+  // blocks that take several tokens: a CTA for each and some of its heads, of k or of v
+  const int per_block = 2 * a.unit_chunks, items = __popc(several) * per_block;
+  for (int i = y; i < items; i += a.unit_ctas_y) {
+    const int from = __fns(several, 0, i / per_block + 1), rest = i % per_block, h = rest / 2 * a.unit_heads;
+    units_of<T, LPR, IL, kCacheThreads>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from),
+                                        from_lane(t.left, from), h, min(h + a.unit_heads, p.num_kv_heads), rest % 2 == 0,
+                                        shared_most);
+    __syncthreads();   // shared_most is the next one's
+  }
+  // single tokens: a warp for each and head
+  const int ones = __popc(single) * per_row;
+  for (int i = y * (kCacheThreads / 32) + warp; i < ones; i += a.unit_ctas_y * (kCacheThreads / 32)) {
+    const int from = __fns(single, 0, i / per_row + 1), rest = i % per_row;
+    units_of<T, LPR, IL, 32>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from), 1, rest / 2,
+                             rest / 2 + 1, rest % 2 == 0, nullptr);
   }
 }
 
-template <typename T, int LPR, bool IL>
-__global__ void __launch_bounds__(kCacheThreads) rotary_cache_kernel(const __grid_constant__ RotaryCache a) {
-  if ((int)blockIdx.x < a.unit_ctas) unit_part<T, LPR, IL>(a);
+// UNITS: 0 none (a cache of 16 bits), 1 of one token each, 2 of up to a block's
+template <typename T, int LPR, bool IL, int UNITS>
+__global__ void __launch_bounds__(kCacheThreads, UNITS == 1 ? 4 : 5) rotary_cache_kernel(const __grid_constant__ RotaryCache a) {
+  if (UNITS && (int)blockIdx.x < a.unit_ctas) unit_part<T, LPR, IL, UNITS == 1>(a);
   else row_part<T, LPR, IL>(a);
 }
 
@@ -429,20 +503,31 @@ int launch_cache(RotaryCache &a, cudaStream_t s) {
   const int heads = p.num_q_heads + (p.key_scales ? 0 : 2 * p.num_kv_heads);
   // heads a thread walks with a token's angles in its registers: up to 8, fewer where the grid would be shallow
   int per = 1;
-  while (per < 8 && groups * ((heads + 2 * per - 1) / (2 * per)) >= 148 * 8 * 4) per *= 2;
-  a.per_cta = per, a.chunks = (heads + per - 1) / per;
+  while (per < 8 && groups * ((heads + 2 * per - 1) / (2 * per)) >= 148 * 16) per *= 2;
+  a.per_cta = per;
+  a.chunks_of[0] = (p.num_q_heads + per - 1) / per;
+  a.chunks_of[1] = a.chunks_of[2] = p.key_scales ? 0 : (p.num_kv_heads + per - 1) / per;
+  a.chunks = a.chunks_of[0] + a.chunks_of[1] + a.chunks_of[2];
   int64_t unit_ctas = 0;
   if (p.key_scales) {
-    const int warps = kCacheThreads / 32, per_row = 2 * p.num_kv_heads;
-    // a tile of rows of prompts has a unit for each block it meets, a tile of single tokens one for each row
-    const int64_t units = (int64_t)per_row * (p.query_starts ? kTile / p.block_size + 2 : kTile);
-    a.unit_ctas_y = (int)((units + warps - 1) / warps);
-    unit_ctas = (int64_t)((p.num_tokens + kTile - 1) / kTile) * a.unit_ctas_y;
+    const int per_row = 2 * p.num_kv_heads;
+    if (!p.query_starts) {
+      unit_ctas = ((int64_t)p.num_tokens * per_row + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
+    } else {
+      // a tile of a prompt's rows has a unit for each block it meets, one of single tokens one for each row: CTAs for the
+      // former, which then take the latter in turn
+      a.unit_heads = 4;
+      a.unit_chunks = (p.num_kv_heads + a.unit_heads - 1) / a.unit_heads;
+      a.unit_ctas_y = 2 * a.unit_chunks * (kTile / p.block_size + 1);
+      unit_ctas = (int64_t)((p.num_tokens + kTile - 1) / kTile) * a.unit_ctas_y;
+    }
   }
   const int64_t grid = unit_ctas + groups * a.chunks;
   if (grid >= (1ll << 31)) return FA_ERR_TOO_LARGE;
   a.unit_ctas = (int)unit_ctas;
-  rotary_cache_kernel<T, LPR, IL><<<(unsigned)grid, kCacheThreads, 0, s>>>(a);
+  auto kern = !p.key_scales ? rotary_cache_kernel<T, LPR, IL, 0>
+              : !p.query_starts ? rotary_cache_kernel<T, LPR, IL, 1> : rotary_cache_kernel<T, LPR, IL, 2>;
+  kern<<<(unsigned)grid, kCacheThreads, 0, s>>>(a);
   FA_CHECK_LAUNCH();
   return FA_OK;
 }
@@ -465,7 +550,8 @@ using namespace fa;
 extern "C" int fa_rotary_cache(const fa_rotary_cache_args *p, void *stream) {
   if (int st = check_cache(p)) return st;
   if (p->num_tokens == 0) return FA_OK;
-  RotaryCache a{*p, 0, 0, 0, 0};
+  RotaryCache a{};
+  a.p = *p;
   auto s = static_cast<cudaStream_t>(stream);
   if (p->dtype == FA_F16) return p->interleaved ? dispatch_cache<__half, true>(a, s) : dispatch_cache<__half, false>(a, s);
   return p->interleaved ? dispatch_cache<__nv_bfloat16, true>(a, s) : dispatch_cache<__nv_bfloat16, false>(a, s);
