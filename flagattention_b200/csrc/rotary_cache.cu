@@ -17,6 +17,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 
@@ -393,11 +394,13 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
     float now = 0.f;
 #pragma unroll 1
     for (int step = 0; step < steps; ++step) {
-      const int pass = step < passes ? step : step - passes;
-      if (passes > 1) u.angles(pass, c, s);
+      const int pass = step < passes ? step : step - passes, next = pass + 1 < passes ? pass + 1 : 0;
       u.values(x, c, s, lo, hi);
-      if (step + 1 < steps) u.load(pass + 1 < passes ? pass + 1 : 0, h, x);
-      else if (h + 1 < h_hi) u.load(0, h + 1, x);
+      // what the next step works on, under the rest of this one
+      if (step + 1 < steps || h + 1 < h_hi) {
+        u.load(next, step + 1 < steps ? h : h + 1, x);
+        if (passes > 1) u.angles(next, c, s);
+      }
       if (step < passes) most = max(most, u.largest(pass, lo, hi));
       if (step == passes - 1) {
         most = __reduce_max_sync(0xffffffffu, most);
@@ -514,12 +517,16 @@ int launch_cache(RotaryCache &a, cudaStream_t s) {
     if (!p.query_starts) {
       unit_ctas = ((int64_t)p.num_tokens * per_row + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
     } else {
-      // a tile of a prompt's rows has a unit for each block it meets, one of single tokens one for each row: CTAs for the
-      // former, which then take the latter in turn
-      a.unit_heads = 4;
+      // A tile of a prompt's rows has a unit for each block it meets, and CTAs for those.  Heads share their rows' angles
+      // where a block is one pass of them and units are many (5800 rows of prompts, 8 heads, us: 70 with a head each, 44
+      // with 4, 46 with 8); longer blocks are work enough.
+      const int64_t tiles = (p.num_tokens + kTile - 1) / kTile, blocks = kTile / p.block_size + 1, ctas = 148 * 5;
+      a.unit_heads = p.block_size <= rows && tiles * blocks * per_row > 2 * ctas ? 4 : 1;
       a.unit_chunks = (p.num_kv_heads + a.unit_heads - 1) / a.unit_heads;
-      a.unit_ctas_y = 2 * a.unit_chunks * (kTile / p.block_size + 1);
-      unit_ctas = (int64_t)((p.num_tokens + kTile - 1) / kTile) * a.unit_ctas_y;
+      // A tile of short sequences has up to a unit of one warp for each row and head: as many CTAs as the GPU has at once.
+      const int64_t most = kTile / (kCacheThreads / 32) * per_row, fill = ctas / tiles;
+      a.unit_ctas_y = (int)std::max(2 * a.unit_chunks * blocks, std::min(most, fill));
+      unit_ctas = tiles * a.unit_ctas_y;
     }
   }
   const int64_t grid = unit_ctas + groups * a.chunks;
