@@ -21,7 +21,6 @@
 #include "paged_parts.cuh"
 
 namespace fa {
-
 // Weights of O run up to 2^(kLift + 8 + 1) and so stay in fp16; the lift keeps 2^kLift more of the small ones above its
 // least number.
 constexpr float kLift = 6.f;
@@ -30,9 +29,12 @@ template <int D>
 struct Paged8Cfg {
   static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
   static constexpr int kWarps = 4;
-  static constexpr int kStages = D <= 128 ? 4 : 3;
-  static constexpr int kTokens = 16;                          // tokens of a group
-  static constexpr int kCtas = D <= 128 ? 3 : 2;   // an SM: a fourth at 128 would spill (428 us for 64 x 1K-32K with 3, 565 with 4)
+  // What is bound here is the issue of instructions, so as many warps as the registers allow and groups that cost few: us
+  // for 64 sequences, 8 kv heads, at 128 (1K-32K tokens): 16 tokens x 3 CTAs 428, x 4 (spills) 565, 32 x 2 481; at 64
+  // (1K-16K): 16 x 3 179, 32 x 3 162, 32 x 4 147, 64 x 2 173.
+  static constexpr int kStages = D <= 64 ? 2 : D <= 128 ? 4 : 3;
+  static constexpr int kTokens = D <= 64 ? 32 : 16;           // tokens of a group
+  static constexpr int kCtas = D <= 64 ? 4 : D <= 128 ? 3 : 2;   // on an SM
   static constexpr int kGroupBytes = kTokens * kD;            // of K or of V
   static constexpr int kStageBytes = 2 * kGroupBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -97,11 +99,12 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  const int seq = blockIdx.x;
+  // the heads of a sequence side by side: their pieces of a block are neighbours in memory
   const int G = a.num_q_heads / a.num_kv_heads;
-  const int q_tiles = (G + 15) / 16;
-  const int hk = blockIdx.y / q_tiles, qt = blockIdx.y % q_tiles;
-  const int part = blockIdx.z;
+  const int q_tiles = (G + 15) / 16, heads = a.num_kv_heads * q_tiles;
+  const int seq = blockIdx.x / heads, head = blockIdx.x % heads;
+  const int hk = head / q_tiles, qt = head % q_tiles;
+  const int part = blockIdx.y;
   const int rows = min(16, G - qt * 16);          // valid query rows of this CTA
   const int qh0 = hk * G + qt * 16;               // first query head
 
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   if (a.partition_size > 0) {
     const LaneLens lens = lane_lens(a, z);   // in flight together with ctx
     if ((long long)part * (z.finest ? z.finest : a.partition_size) >= ctx) return;
-    const int size = partition_tokens(a, z, lens, ctx, gridDim.z);
+    const int size = partition_tokens(a, z, lens, ctx, gridDim.y);
     if ((long long)part * size >= ctx) return;
     t_begin = part * size;
     t_end = (int)min((long long)ctx, (long long)t_begin + size);
@@ -547,7 +550,7 @@ static int launch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_
   if (int st = ensure_dyn_smem(kern, C::kTotal, &attr_done)) return st;
   const int q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;
   const int P = a->partition_size > 0 ? (a->max_context_len + a->partition_size - 1) / a->partition_size : 1;
-  kern<<<dim3(a->num_seqs, a->num_kv_heads * q_tiles, P), C::kWarps * 32, C::kTotal, stream>>>(*p, z);
+  kern<<<dim3(a->num_seqs * a->num_kv_heads * q_tiles, P), C::kWarps * 32, C::kTotal, stream>>>(*p, z);
   FA_CHECK_LAUNCH();
   return FA_OK;
 }

@@ -57,7 +57,7 @@ def coarsen_partition(partition_size, pairs, context_len, num_sms, most=2048):
 
 
 @functools.lru_cache(maxsize=1024)
-def size_partitions(base, num_seqs, ctas, max_context_len, num_sms):
+def size_partitions(base, num_seqs, ctas, max_context_len, num_sms, fill=0.8, many=35, top=2048, slots=0):
     """(workspace partition, finest, coarsest, ctas, parts) of a fa_paged_attention call: how far partitions of `base`
     tokens may grow when max_context_len is an upper bound and lengths differ.  `ctas`: CTAs that a partition of one
     sequence takes; workspace partition 0: one pass does it.
@@ -72,20 +72,29 @@ def size_partitions(base, num_seqs, ctas, max_context_len, num_sms):
                    64 x 32768 at most 852 / 642 / 647, 64 x 8192 at most 233 / 189 / 192, 4 x 32768 at most 103 / 74 / 75
       2 kv heads   4 x 1500 under 32768 9.5 / 21 / 10.3, 4096 and 63 x 200 16.5 / 26 / 17.5, 16 x 32768 at most
                    96 / 52 / 55, 32768 and 15 x 1000 44 / 33 / 32, 64 x 32768 at most 253 / 159 / 174"""
+    pairs = num_seqs * ctas
+    if 16 * pairs <= slots * num_sms < pairs * _cdiv(max_context_len, base):
+        # few long contexts: one wave of equal partitions, `slots` CTAs an SM (131071 tokens, 8 kv heads, codes of 8 bits: 59
+        # us so, 76 with the power of two below, 71 with the one above)
+        parts = slots * num_sms // pairs
+        finest = size = max(base, _cdiv(_cdiv(max_context_len, parts), 128) * 128)
+        while finest % 32 == 0 and finest >= 256:   # for contexts far below the bound
+            finest //= 2
+        return (0, base, base, 0, 1) if max_context_len <= size else (size, finest, size, 0, parts)
     coarsest = base
-    while coarsest < 2048:
+    while coarsest < top:
         coarsest *= 2
     size = base
-    while size < coarsest and (ctas * _cdiv(max_context_len, 2 * size) >= 0.8 * num_sms
-                               or num_seqs * ctas * _cdiv(max_context_len, size) > 35 * num_sms):
+    while size < coarsest and (ctas * _cdiv(max_context_len, 2 * size) >= fill * num_sms
+                               or num_seqs * ctas * _cdiv(max_context_len, size) > many * num_sms):
         size *= 2
     if max_context_len <= size:
         return 0, base, coarsest, 0, 1
     pairs = num_seqs * ctas
     by_length = (size < min(coarsest, 4 * base) and num_seqs <= 2048
-                 and pairs * _cdiv(max_context_len, 2 * size) >= 0.8 * num_sms)
+                 and pairs * _cdiv(max_context_len, 2 * size) >= fill * num_sms)
     if by_length:
-        return size, base, coarsest, int(0.8 * num_sms), 0
+        return size, base, coarsest, int(fill * num_sms), 0
     return size, base if pairs < 2 * num_sms else size, coarsest, 0, max(1, _cdiv(2 * num_sms, pairs))
 
 
@@ -99,22 +108,22 @@ def partition_workspace(rows, P, D, device):
     return ws, base, part_max, part_max + stats * 4
 
 
-def _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms):
+def _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms, how=()):
     """(partition size, partitions of the workspace, sizing or None) of a call; partition size 0: one pass."""
     # kept for plain numbers only: a tensor hashes by identity, and its value may change
     plan = _kept_plan if type(num_splits) is int else _kept_plan.__wrapped__
-    return plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms)
+    return plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms, how)
 
 
 @functools.lru_cache(maxsize=1024)
-def _kept_plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms):
+def _kept_plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits, num_sms, how=()):
     free_choice = num_splits == 0
     num_splits, partition_size = plan_partitions(num_seqs, num_kv_heads, kv_block_size, max_context_len, num_splits,
                                                  num_sms)
     sizing = None
     if free_choice and partition_size:
         partition_size, *sizing = size_partitions(
-            partition_size, num_seqs, num_kv_heads * _cdiv(num_q_heads // num_kv_heads, 16), max_context_len, num_sms)
+            partition_size, num_seqs, num_kv_heads * _cdiv(num_q_heads // num_kv_heads, 16), max_context_len, num_sms, *how)
     if not partition_size:
         return 0, 0, None
     return partition_size, _cdiv(max_context_len, partition_size), sizing
@@ -277,6 +286,15 @@ def _stride(t, i):
     return t.stride(i) if t.shape[i] > 1 else 0
 
 
+def _how_8bit(head_size):
+    """(fill, many, top, slots) of size_partitions for caches of 8 bits.
+
+    A token's bytes are half and a CTA's work on it is not, so partitions end where more CTAs an SM are at hand, and
+    may be longer: 16-bit rule -> this, us: 37 x 1-8191 tokens, 2 kv heads of 16, head 64 34 -> 25, 64 x 1K-32K, 8 kv
+    heads of 4, head 128 439 -> 422, 2 x 8000 19.6 -> 15."""
+    return 3, 35, 4096, 4 if head_size <= 64 else 3 if head_size <= 128 else 2
+
+
 def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
                    max_context_len, num_splits=0):
     """`attention` over caches held in 8 bits: key_cache, value_cache [num_blocks, kv_heads, block, head] of
@@ -313,7 +331,7 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
         return out
     with _C.device_guard(query.device):
         partition_size, P, sizing = _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits,
-                                          _C.sm_count(query.device))
+                                          _C.sm_count(query.device), _how_8bit(head_size))
         part_out = part_max = part_sum = 0
         if partition_size:
             assert partition_size % 16 == 0, f"partition_size={partition_size}"
@@ -336,12 +354,12 @@ def _native_8bit(query, key_cache, value_cache, key_scales, value_scales, contex
     """The call through native code, or None; the partitions are chosen here."""
     if query.dim() != 3 or key_cache.dim() != 4:
         return None
-    num_seqs, num_q_heads, _ = query.shape
+    num_seqs, num_q_heads, head_size = query.shape
     num_kv_heads, kv_block_size = key_cache.shape[1:3]
     if not num_seqs or not num_q_heads or not num_kv_heads or num_q_heads % num_kv_heads or not kv_block_size:
         return None
     partition_size, P, sizing = _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, 0,
-                                      _C.sm_count(query.device))
+                                      _C.sm_count(query.device), _how_8bit(head_size))
     return _native.load().paged_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
                                      attn_scale, max_context_len, partition_size, P, *(sizing or (0, 0, 0, 0)))
 

@@ -114,7 +114,8 @@ def test_rotary_and_cache(python_form, held, starts):  # noqa: F811
 def test_paged_8bit(python_form, most):  # noqa: F811
     x = [t.cuda() for t in made_decode([300, 0, 17], 16, 2, 128, 16, torch.bfloat16)]
     call = lambda: fa.paged_attention_8bit(*x, 0.1, most)  # noqa: E731
-    P = paged._plan(3, 16, 2, 16, most, 0, torch.cuda.get_device_properties(0).multi_processor_count)
+    P = paged._plan(3, 16, 2, 16, most, 0, torch.cuda.get_device_properties(0).multi_processor_count,
+                    paged._how_8bit(128))
     assert _native.load().paged_8bit(*x, 0.1, most, P[0], P[1], *(P[2] or (0, 0, 0, 0))) is not None
     _same([call()], [python_form(call)])
 

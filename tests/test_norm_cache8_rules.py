@@ -170,6 +170,29 @@ def test_packed_structs():
     assert (got.key_scales, got.value_scales, got.num_blocks, got.table_cols) == (100, 101, 102, 103)
 
 
+def test_partitions_of_8_bit_calls_are_what_the_library_takes():
+    """Sizes nest, cover the bound and are whole groups of tokens, for any call (paged_parts.cuh: sizing_ok)."""
+    import random
+    from flagattention_b200 import paged
+    rng = random.Random(1)
+    for _ in range(3000):
+        Hk = rng.choice([1, 2, 4, 5, 8])
+        seqs, G, D = rng.choice([1, 2, 3, 8, 37, 64, 300, 3000]), rng.choice([1, 4, 8, 16, 17, 40]), rng.choice([16, 64, 128, 256])
+        block, most = rng.choice([16, 32, 48, 128, 512]), int(2 ** rng.uniform(0, 20))
+        size, P, sizing = paged._plan(seqs, G * Hk, Hk, block, most, 0, 148, paged._how_8bit(D))
+        if not size:
+            assert sizing is None
+            continue
+        finest, coarsest, ctas, parts = sizing
+        assert P * size >= most > (P - 1) * size and size % 16 == finest % 16 == 0 and 0 < finest <= size
+        for x in (size, coarsest):
+            assert x % finest == 0 and (x // finest) & (x // finest - 1) == 0 and x >= finest
+        assert ctas >= 0 and (ctas > 0 or parts > 0) and (ctas == 0 or seqs <= 2048)
+    # one long context: one wave of CTAs
+    size, P, sizing = paged._plan(1, 64, 8, 32, 131072, 0, 148, paged._how_8bit(128))
+    assert 8 * P <= 3 * 148 < 8 * P * 2 and sizing[3] == 55
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     """The checks behind `is_cuda`, with nothing launched."""
