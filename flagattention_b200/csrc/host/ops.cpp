@@ -679,7 +679,7 @@ bool lengths_ready(const Tensor &t, int64_t n, int device) {
   return plain(t, device) && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
 bool block_table_ready(const Tensor &t, int64_t seqs, int device) {
-  return plain(t, device) && integers(t) && t.dim() == 2 && t.size(0) == seqs && t.size(1) <= INT_MAX &&
+  return plain(t, device) && integers(t) && t.dim() == 2 && t.size(0) == seqs && t.size(1) <= INT_MAX && t.numel() > 0 &&
          (t.stride(1) == 1 || t.size(1) <= 1);
 }
 int64_t stride(const Tensor &t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; }

@@ -17,6 +17,8 @@
 // weights stay in range whatever the scales are (0 too: E = -inf).
 // bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): elements down to 2^-38 of
 // the maximum keep their bits or lose less than 2^-40 of it.
+#include <climits>
+
 #include "common.cuh"
 #include "paged_parts.cuh"
 
@@ -521,7 +523,7 @@ static int validate_8bit(const fa_paged_8bit_args *p) {
     return FA_ERR_BAD_ARG;
   if (a->dtype != FA_F16 && a->dtype != FA_BF16) return FA_ERR_BAD_ARG;
   if (a->num_seqs <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->block_size <= 0 ||
-      a->max_context_len <= 0 || a->partition_size < 0 || p->num_blocks < 0 || p->table_cols < 0)
+      a->max_context_len <= 0 || a->partition_size < 0 || p->num_blocks < 0 || p->table_cols <= 0)
     return FA_ERR_BAD_ARG;
   if (a->num_q_heads % a->num_kv_heads != 0 || a->block_size % 16 != 0 || a->partition_size % 16 != 0 ||
       a->causal_rows != 0 || (a->block_table_is_i64 != 0 && a->block_table_is_i64 != 1))
@@ -535,7 +537,7 @@ static int validate_8bit(const fa_paged_8bit_args *p) {
     return FA_ERR_ALIGNMENT;
   if (a->partition_size > 0 && (!a->part_out || !a->part_max || !a->part_sum)) return FA_ERR_WORKSPACE;
   const int64_t q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;   // (what a grid holds)
-  if (a->num_kv_heads * q_tiles > 65535 || a->num_q_heads > 65535 ||
+  if (a->num_q_heads > 65535 || (int64_t)a->num_seqs * a->num_kv_heads * q_tiles > INT_MAX ||
       (a->partition_size > 0 && (a->max_context_len - 1) / a->partition_size >= 65535))
     return FA_ERR_TOO_LARGE;
   return FA_OK;

@@ -254,6 +254,7 @@ def _check_scales(key_cache, key_scales, value_scales):
 def _check_caches(key_cache, value_cache, num_kv_heads, head_size, unit):
     """What both writers and readers of caches with a table ask: `unit` elements are 16 bytes."""
     assert key_cache.dim() == 4 and key_cache.shape == value_cache.shape
+    assert key_cache.shape[0] > 0, "caches have blocks"
     assert key_cache.shape[1] == num_kv_heads and key_cache.shape[3] == head_size
     assert key_cache.dtype == value_cache.dtype
     assert key_cache.device == value_cache.device, "the caches are on one device"
@@ -327,8 +328,8 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
     block_tables = _table_ready(block_tables, num_seqs, query.device)
     query = _rows_ready(query)
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    if num_seqs == 0:
-        return out
+    if num_seqs == 0 or block_tables.shape[1] == 0:
+        return out.zero_()
     with _C.device_guard(query.device):
         partition_size, P, sizing = _plan(num_seqs, num_q_heads, num_kv_heads, kv_block_size, max_context_len, num_splits,
                                           _C.sm_count(query.device), _how_8bit(head_size))
@@ -426,6 +427,8 @@ def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, bl
     out = torch.empty(query.shape, dtype=query.dtype, device=device)
     if num_tokens == 0:
         return out
+    if num_seqs == 0 or block_tables.shape[1] == 0:   # no row has a place
+        return out.zero_()
 
     def ptr(t):
         return 0 if t is None else t.data_ptr()

@@ -2,7 +2,7 @@
 
 The step between a decoder's projections and flash_attention.  No reference counterpart: its operators take queries and
 keys as they are.  One HBM-bound launch forward for q and k together; one backward, and a small one that adds up the
-weights' gradients, in an order that depends on the shape alone.
+weights' gradients, in an order that depends on the shape and the GPU's number of SMs: the same bits every time.
 """
 import torch
 

@@ -13,7 +13,8 @@ import torch
 
 from .dropout import recompute_mask  # noqa: F401
 
-__all__ = ["flash_attention", "piecewise_attention", "paged_attention", "recompute_mask", "rotary_pair"]
+__all__ = ["flash_attention", "piecewise_attention", "paged_attention", "paged_attention_8bit", "qk_norm_rotary",
+           "recompute_mask", "rotary_pair"]
 
 
 def _causal_mask(m, n, device):
@@ -99,3 +100,44 @@ def rotary_pair(x, cos1, sin1, cos2, sin2, positions=None, interleaved=False, up
         return y.to(x.dtype)
 
     return one(cos1, sin1), one(cos2, sin2)
+
+
+def paged_attention_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, scale):
+    """PyTorch reference of flagattention_b200.paged_attention_8bit, in fp32."""
+    def held(codes, scales):   # the blocks that tables name, as numbers
+        return codes.view(torch.uint8)[ids].view(codes.dtype).float() * scales[ids][:, :, None, None]
+
+    out = torch.zeros_like(query)
+    kv_heads, block, head = key_cache.shape[1:]
+    for i, ctx in enumerate(context_lens.tolist()):
+        if ctx <= 0:
+            continue
+        ids = block_tables[i, : (ctx + block - 1) // block].long()
+        kk = held(key_cache, key_scales).transpose(0, 1).reshape(kv_heads, -1, head)[:, :ctx]
+        vv = held(value_cache, value_scales).transpose(0, 1).reshape(kv_heads, -1, head)[:, :ctx]
+        qq = query[i].float().view(kv_heads, -1, head)
+        p = torch.softmax(torch.bmm(qq, kk.transpose(1, 2)) * scale, dim=-1)
+        out[i] = torch.bmm(p, vv).reshape(-1, head).to(out.dtype)
+    return out
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, interleaved=False, eps=1e-6, upcast=True):
+    """PyTorch reference of flagattention_b200.qk_norm_rotary, differentiable through autograd.
+    upcast=False does the arithmetic in q's own dtype (the same-precision comparison)."""
+    half = cos.shape[1]
+    if positions is None:
+        positions = torch.arange(q.shape[2], device=q.device)
+    rows = positions.to(device=cos.device, dtype=torch.int64).reshape(-1, q.shape[2]).clamp(0, cos.shape[0] - 1)
+
+    def one(x, weight):
+        work = x.float() if upcast else x
+        c, s = (t[rows][:, None].to(device=x.device, dtype=work.dtype) for t in (cos, sin))
+        n = work * torch.rsqrt(work.float().square().mean(-1, keepdim=True) + eps).to(work.dtype)
+        if weight is not None:
+            n = n * weight.to(work.dtype)
+        lo, hi = (n[..., 0:2 * half:2], n[..., 1:2 * half:2]) if interleaved else (n[..., :half], n[..., half:2 * half])
+        ylo, yhi = lo * c - hi * s, hi * c + lo * s
+        y = torch.stack((ylo, yhi), dim=-1).flatten(-2) if interleaved else torch.cat((ylo, yhi), dim=-1)
+        return torch.cat((y, n[..., 2 * half:]), dim=-1).to(x.dtype)
+
+    return one(q, q_weight), one(k, k_weight)

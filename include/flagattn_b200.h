@@ -426,7 +426,7 @@ int fa_qk_norm_rotary_fwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, con
 /* Its backward from q, k and the gradients gq, gk of the results: dq, dk, and dq_weight, dk_weight (of the
  * weights' type; NULL = not wanted).  The weights' gradients go by a workspace of
  * fa_qk_norm_rotary_bwd_workspace_bytes (not needed where both are NULL) and are added in an order that depends on
- * the shape alone. */
+ * the shape and the number of SMs.  The size is asked for on the device of the call. */
 int64_t fa_qk_norm_rotary_bwd_workspace_bytes(const fa_norm_rotary_args *a);
 int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, const fa_tensor4 *k, const fa_tensor4 *gq,
                           const fa_tensor4 *gk, const fa_tensor4 *dq, const fa_tensor4 *dk, void *dq_weight,
@@ -473,7 +473,7 @@ int fa_rotary_cache(const fa_rotary_cache_args *a, void *stream);
 
 /* fa_paged_decode over caches of e4m3 codes (strides in codes, multiples of 16) with fp32 scales (num_blocks,
  * num_kv_heads), contiguous, 0 or positive: value = code * scale.  `paged` as for fa_paged_decode, with
- * block_size a multiple of 16, causal_rows 0 and a block table of `table_cols` columns.  partition_size 0: one
+ * block_size a multiple of 16, causal_rows 0 and a block table of `table_cols` >= 1 columns.  partition_size 0: one
  * pass; otherwise partial results in the workspace and their reduction, with partitions of partition_size tokens
  * (finest 0) or sized on the GPU as in fa_paged_attention.  A block id outside [0, num_blocks) makes its sequence's
  * output NaN. */

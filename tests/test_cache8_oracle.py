@@ -38,3 +38,26 @@ def test_backward_against_autograd_in_64_bits():
         da, db = torch.autograd.grad(y, (a, b), g)
         dx, dw, _, _ = cache8.norm_rotary_backward(x, w, g, cos, sin, pos, inter)
         assert torch.allclose(dx, da, rtol=1e-10, atol=1e-12) and torch.allclose(dw, db, rtol=1e-10, atol=1e-12)
+
+
+def test_shipped_references_say_the_same():
+    """flagattention_b200.testing in fp32 against the 64-bit statements: a rounding of the output apart."""
+    import flagattention_b200 as fa
+    gen = torch.Generator().manual_seed(3)
+    q, k = torch.randn(2, 4, 9, 32, generator=gen).half(), torch.randn(2, 2, 9, 32, generator=gen).half()
+    wq, wk = torch.randn(32, generator=gen), torch.randn(32, generator=gen)
+    cos, sin = fa.rotary_tables(20, 16)
+    pos = torch.randint(-2, 30, (2, 9), generator=gen)
+    for inter in (False, True):
+        y = fa.testing.qk_norm_rotary(q, k, wq, wk, cos, sin, pos, inter)
+        for a, x, w in zip(y, (q, k), (wq, wk)):
+            want = cache8.norm_rotary(x, w, cos, sin, pos, inter)
+            # (half a step of fp16, and some twenty fp32 roundings of terms below 16)
+            assert ((a.double() - want).abs() <= 2.0 ** -11 * want.abs() + 32 * 16 * 2.0 ** -24).all()
+    codes = [torch.randn(7, 2, 16, 32, generator=gen).to(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.rand(7, 2, generator=gen) for _ in range(2)]
+    bt = torch.randperm(7, generator=gen)[:6].view(2, 3)
+    lens, qq = torch.tensor([40, 0]), torch.randn(2, 4, 32, generator=gen).half()
+    got = fa.testing.paged_attention_8bit(qq, *codes, *scales, lens, bt, 0.2)
+    want, size, _ = cache8.paged_attention_8bit(qq, *codes, *scales, lens, bt, 0.2)
+    assert ((got.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -16 * size).all() and (got[1] == 0).all()

@@ -132,7 +132,7 @@ def test_library_checks_rotary_cache(built_lib):
 def test_library_checks_paged_8bit(built_lib):
     lib = _C.load()
 
-    def call(sizing=(0, 0, 0, 0), key_scales=0x1000, num_blocks=4, **change):
+    def call(sizing=(0, 0, 0, 0), key_scales=0x1000, num_blocks=4, table_cols=2, **change):
         a = _C.Paged8bitArgs()
         base = dict(dtype=_C.FA_F16, num_seqs=3, num_q_heads=4, num_kv_heads=2, head_size=64, block_size=16,
                     max_context_len=512, query=0x1000, key_cache=0x1000, value_cache=0x1000, context_lens=0x1000,
@@ -140,7 +140,7 @@ def test_library_checks_paged_8bit(built_lib):
         base.update(change)
         for n, v in base.items():
             setattr(a.paged, n, v)
-        a.key_scales, a.value_scales, a.num_blocks, a.table_cols = key_scales, 0x1000, num_blocks, 2
+        a.key_scales, a.value_scales, a.num_blocks, a.table_cols = key_scales, 0x1000, num_blocks, table_cols
         return lib.fa_paged_attention_8bit(ctypes.byref(a), *sizing, None)
 
     parts = dict(partition_size=256, part_out=0x1000, part_max=0x1000, part_sum=0x1000)
@@ -150,7 +150,8 @@ def test_library_checks_paged_8bit(built_lib):
                            (dict(head_size=48), -2), (dict(head_size=512), -2), (dict(key_cache=0x1008), -3),
                            (dict(kv_stride_t=8), -3), (dict(q_stride_h=12), -3), (dict(partition_size=256), -5),
                            (dict(context_lens=None), -1), (dict(key_scales=None), -1), (dict(num_blocks=-1), -1),
-                           (dict(num_q_heads=200000, num_kv_heads=100000), -6)):
+                           (dict(num_q_heads=200000, num_kv_heads=100000), -6), (dict(table_cols=0), -1),
+                           (dict(num_seqs=1 << 27, num_q_heads=64, num_kv_heads=32), -6)):
         assert call(**change) == status, change
     for sizing in ((24, 256, 0, 1), (256, 128, 0, 1), (96, 256, 0, 1), (256, 512, -1, 1), (256, 512, 0, 0)):
         assert call(sizing, **parts) == -1, sizing

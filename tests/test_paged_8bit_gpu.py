@@ -174,6 +174,24 @@ def test_a_cache_beyond_32_bits():
     check(out, x, D ** -0.5)
 
 
+def test_tables_without_columns_and_no_sequences():
+    x = [t.cuda() for t in made([40, 3], 4, 2, 64, 16, torch.float16)]
+    assert (fa.paged_attention_8bit(*x[:6], x[6][:, :0], 0.125, 40) == 0).all()
+    assert fa.paged_attention_8bit(x[0][:0], *x[1:5], x[5][:0], x[6][:0], 0.125, 40).shape == (0, 4, 64)
+    x[5].fill_(-3)       # no length
+    assert (fa.paged_attention_8bit(*x, 0.125, 40) == 0).all() and (fa.paged_attention_8bit(*x, 0.125, 9000) == 0).all()
+
+
+def test_a_table_narrower_than_the_lengths():
+    """Tokens without a column of the table are not there."""
+    x = made([100, 64], 4, 2, 64, 16, torch.float16, seed=3)
+    short = (*x[:6], x[6][:, :4].contiguous())
+    same = (*x[:5], torch.tensor([64, 64], dtype=torch.int32), short[6])
+    assert torch.equal(call(short, 0.125, 100, 1), call(same, 0.125, 100, 1))
+    for most, splits in ((100, 2), (100, 0), (9000, 0)):
+        check(call(short, 0.125, most, splits), same, 0.125)
+
+
 def test_ids_outside_the_cache_give_nan_and_nothing_else():
     x = made([100, 100, 40], 4, 2, 64, 16, torch.float16, seed=3)
     good = call(x, 0.125, 100)

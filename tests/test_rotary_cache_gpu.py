@@ -237,6 +237,26 @@ def test_empty_call():
     b.check(b.call(d), d)
 
 
+@pytest.mark.parametrize("held", [True, False])
+def test_rows_without_sequences_or_tables(held):
+    """No sequence at all, and tables without a column: queries of 0, caches as they were."""
+    b = Batch([], [], 4, 2, 64, 16, torch.bfloat16, held, seed=3, pad=7)
+    d = b.device()
+    assert d["lens"].numel() == 0
+    out = b.call(d)
+    assert out.shape == (7, 4, 64) and (out == 0).all()
+    b = Batch([0, 0], [1, 1], 4, 2, 64, 16, torch.bfloat16, held, seed=3)
+    b.table = b.table[:, :0]
+    d = b.device()
+    assert (b.call(d) == 0).all()
+    assert torch.equal(d["kc"].cpu(), b.kc)
+    b = Batch([3, 9], [4, 2], 4, 2, 64, 16, torch.bfloat16, held, seed=3)
+    b.starts += 5        # rows in front of the first sequence
+    b.qkv = torch.cat((b.qkv[:5], b.qkv))
+    d = b.device()
+    b.check(b.call(d), d)
+
+
 def test_captured_step_follows_lengths():
     b = Batch([15, 3, 40], [1, 1, 1], 4, 2, 128, 16, torch.bfloat16, True, seed=6, starts=False, cols=5)
     b.cos, b.sin = fa.rotary_tables(100, 128)
