@@ -41,8 +41,8 @@ struct Paged8Cfg {
   static constexpr int kStageBytes = 2 * kGroupBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kQBytes = 16 * kD * 2;
-  static constexpr int kScales = kQBytes;                     // per warp and stage: K, V of the first 16 tokens, K, V of the others
-  static constexpr int kRowScale = kScales + kWarps * kStages * 16;
+  static constexpr int kScales = kQBytes;                     // per warp: of 64 pieces, K and V
+  static constexpr int kRowScale = kScales + kWarps * 64 * 8;
   static constexpr int kStats = kRowScale + 16 * 4;           // per warp and row: maximum, sum, reference of O
   static constexpr int kRing = (kStats + 3 * kWarps * 16 * 4 + 127) / 128 * 128;
   static constexpr int kRingBytes = kWarps * kWarpBytes;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   const int n_groups = t_end > t_begin ? (t_end - t_begin + GT - 1) / GT : 0;
   const int my_groups = n_groups > warp ? (n_groups - warp + NW - 1) / NW : 0;
   const uint32_t ring = smem + C::kRing + warp * C::kWarpBytes;
-  const uint32_t scales = smem + C::kScales + warp * NS * 16;
+  const uint32_t scales = smem + C::kScales + warp * 64 * 8;
   const uint8_t *kc = static_cast<const uint8_t *>(a.key_cache) + (int64_t)hk * a.kv_stride_h;
   const uint8_t *vc = static_cast<const uint8_t *>(a.value_cache) + (int64_t)hk * a.kv_stride_h;
   const int64_t v_minus_k = vc - kc;
@@ -141,43 +141,66 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   for (int c = 0; c < NC; ++c) dst_off[c] = code_offset<KD>(c * RPC + lane_r, ch);
   const int64_t lane_src = (int64_t)lane_r * a.kv_stride_t + ch * 16;
 
-  // blocks of the 16-token pieces of this warp's i-th group, looked up a group ahead of their use; -1 where the piece
-  // holds no token of the partition, -2 for an id outside the cache
-  int64_t next[NH];
-  auto look_up = [&](int i) {
-#pragma unroll
-    for (int s = 0; s < NH; ++s) {
-      const int tok = t_begin + (warp + i * NW) * GT + 16 * s;
-      next[s] = -1;
-      if (i < my_groups && tok < t_end) {
-        const int64_t id = phys_block<IdxT>(a.block_tables, a.bt_stride_s, seq, bs_shift >= 0 ? tok >> bs_shift : tok / BS);
-        next[s] = id >= 0 && id < p.num_blocks ? id : -2;
-      }
-    }
+  // Where the warp's 16-token pieces lie is worked out for 32 of them at a time, one a lane, and handed on by shuffles: the
+  // table, its bounds and the 64-bit products would otherwise be a sixth of a group's instructions.
+  const auto piece_tok = [&](int q) { return t_begin + (warp + q / NH * NW) * GT + 16 * (q % NH); };
+  IdxT id_ahead = 0;   // of the 32 pieces behind those of `place`
+  int64_t place = -1;  // byte offset of this lane's piece; -1: without a token, -2: its id is outside the cache
+  const auto look_up = [&](int q0) {
+    const int q = q0 + lane, tok = piece_tok(q);
+    if (q < my_groups * NH && tok < t_end)
+      id_ahead = static_cast<const IdxT *>(a.block_tables)[(int64_t)seq * a.bt_stride_s + (bs_shift >= 0 ? tok >> bs_shift : tok / BS)];
   };
+  const auto settle = [&](int q0) {   // the next 32 pieces: their places, their scales into shared memory
+    const int q = q0 + lane, tok = piece_tok(q);
+    const bool here = q < my_groups * NH && tok < t_end, ok = here && id_ahead >= 0 && id_ahead < p.num_blocks;
+    const int in_blk = bs_shift >= 0 ? tok & (BS - 1) : tok % BS;
+    place = ok ? (int64_t)id_ahead * a.kv_stride_b + (int64_t)in_blk * a.kv_stride_t : here ? -2 : -1;
+    const uint32_t at = scales + (q & 63) * 8;
+    if (ok) {
+      const int64_t from = (int64_t)id_ahead * a.num_kv_heads + hk;
+      cp_async4(at, p.key_scales + from);
+      cp_async4(at + 4, p.value_scales + from);
+    } else {   // a block outside the cache makes its sequence's output NaN; a piece without tokens counts as nothing
+      const float none = here ? NAN : 0.f;
+      asm volatile("st.shared.v2.f32 [%0], {%1, %1};\n" ::"r"(at), "f"(none) : "memory");
+    }
+    look_up(q0 + 32);
+  };
+  const uint8_t *k_lane = kc + lane_src;
   const int64_t c_step = (int64_t)RPC * a.kv_stride_t;
-  auto issue = [&](int i) {   // i-th group of this warp -> stage i % NS
+  const bool packed = a.kv_stride_t == D;   // steps that are known when this is compiled
+  const auto issue = [&](int i) {   // i-th group of this warp -> stage i % NS
+    if (i * NH % 32 == 0) settle(i * NH);
     const int tok0 = t_begin + (warp + i * NW) * GT;
     const uint32_t st = ring + (i % NS) * C::kStageBytes;
-    int64_t blk[NH];
-    const uint8_t *src[NH];
+    int64_t at[NH];
     bool whole = tok0 + GT <= t_end;
 #pragma unroll
     for (int s = 0; s < NH; ++s) {
-      blk[s] = next[s];
-      whole = whole && blk[s] >= 0;
-      const int tok = tok0 + 16 * s;
-      const int in_blk = bs_shift >= 0 ? tok & (BS - 1) : tok % BS;
-      src[s] = kc + max(blk[s], (int64_t)0) * a.kv_stride_b + (int64_t)in_blk * a.kv_stride_t + lane_src;
+      at[s] = __shfl_sync(0xffffffffu, place, (i * NH + s) % 32);
+      whole = whole && at[s] >= 0;
     }
-    look_up(i + 1);
-    if (RPC <= 16 && whole) {
+    if (RPC <= 16 && whole && packed) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const uint8_t *&from = src[c * RPC / 16];
-        cp_async16(st + dst_off[c], from, true);
-        cp_async16(st + C::kGroupBytes + dst_off[c], from + v_minus_k, true);
-        from += c_step;
+      for (int s = 0; s < NH; ++s) {
+        const uint8_t *sk = k_lane + at[s], *sv = sk + v_minus_k;
+#pragma unroll
+        for (int c = s * (NC / NH); c < (s + 1) * (NC / NH); ++c) {
+          cp_async16(st + dst_off[c], sk + c * RPC % 16 * D, true);
+          cp_async16(st + C::kGroupBytes + dst_off[c], sv + c * RPC % 16 * D, true);
+        }
+      }
+    } else if (RPC <= 16 && whole) {
+#pragma unroll
+      for (int s = 0; s < NH; ++s) {
+        const uint8_t *sk = k_lane + at[s];
+#pragma unroll
+        for (int c = s * (NC / NH); c < (s + 1) * (NC / NH); ++c) {
+          cp_async16(st + dst_off[c], sk, true);
+          cp_async16(st + C::kGroupBytes + dst_off[c], sk + v_minus_k, true);
+          sk += c_step;
+        }
       }
     } else {
 #pragma unroll
@@ -188,8 +211,8 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
 #pragma unroll
         for (int k = 0; k < NH; ++k)
           if (s == k) {
-            ok = ok && blk[k] >= 0;
-            sk = src[k] + (int64_t)(RPC <= 16 ? c * RPC % 16 : -16 * k) * a.kv_stride_t;
+            ok = ok && at[k] >= 0;
+            sk = k_lane + at[k] + (int64_t)(RPC <= 16 ? c * RPC % 16 : -16 * k) * a.kv_stride_t;
           }
         if (s >= NH) ok = false;
         if (!ok) sk = kc;
@@ -198,14 +221,6 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
           cp_async16(st + C::kGroupBytes + dst_off[c], sk + v_minus_k, ok);
         }
       }
-    }
-    if (lane < 2 * NH) {
-      const uint32_t at = scales + (i % NS) * 16 + lane * 4;
-      const int64_t id = blk[NH > 1 && lane >= 2 ? 1 : 0];
-      const float *from = lane & 1 ? p.value_scales : p.key_scales;
-      if (id >= 0) cp_async4(at, from + id * a.num_kv_heads + hk);
-      // a block outside the cache makes its sequence's output NaN; a piece without tokens counts as nothing
-      else asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(at), "f"(id == -2 ? NAN : 0.f) : "memory");
     }
   };
 
@@ -306,7 +321,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
     float ks[NH], ve[NH], vf[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      const uint2 sc = lds8(scales + (i % NS) * 16 + 8 * h);
+      const uint2 sc = lds8(scales + (i * NH + h) % 64 * 8);
       ks[h] = __uint_as_float(sc.x);
       split_scale(__uint_as_float(sc.y), ve[h], vf[h]);
     }
