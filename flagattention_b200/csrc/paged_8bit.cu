@@ -1,14 +1,17 @@
 // paged_attention_8bit decode: paged.cu's gather over a cache of e4m3 codes with an fp32 scale for each block and kv head.
 //
-// HBM-bound as there: every warp streams groups of codes and their scales through a cp.async ring of its own.
-// Codes go to fp16 (exactly) on the way from shared memory to the tensor cores, and two things follow from bytes:
-//  * S = Q K^T contracts over the head, in whatever order both operands agree on: a lane takes 16 codes that lie side by
-//    side as four steps of its K fragment, so K needs neither ldmatrix nor a transposition, and Q's fragments are read
-//    in that order.
-//  * O = P V contracts over tokens, whose codes lie apart: a lane reads the same 16 head elements of four tokens and
-//    interleaves them two by two (one byte permutation for two conversions). Columns of the accumulator are head
-//    elements in that order, so a lane ends with consecutive ones.
-// Which 8 tokens a fragment's columns mean (token_of) and where a row's 16-byte pieces lie (code_offset) are chosen so that
+// Bytes are half of that and products are not, so instructions count: every warp streams groups of codes through a
+// cp.async ring of its own, and codes, turned to fp16 exactly on their way from shared memory, are the left operands of both
+// products, S^T = K Q^T and O^T = V^T P^T.  Queries are the 8 columns of a fragment, so that a group of 8 heads or fewer
+// wastes nothing (as 16 rows of the left operand they fill half of it and need twice the accumulators: 12 warps an SM
+// instead of 16, 64 sequences of 1K-32K tokens 381 us instead of 355).
+//  * S^T contracts over the head, in whatever order both operands agree on: a lane takes 16 codes that lie side by side as
+//    four steps of its K fragment, so K needs neither ldmatrix nor a transposition, and Q's fragments are read in that
+//    order.
+//  * O^T contracts over tokens, whose codes lie apart: a lane reads the same 16 head elements of four tokens and
+//    interleaves them two by two (one byte permutation for two conversions).  Rows of the accumulator are head elements in
+//    that order, so a lane ends with consecutive ones.  P^T comes from S^T by transposing 8 x 8 tiles in registers.
+// Which 8 tokens a fragment's rows mean (token_of) and where a row's 16-byte pieces lie (code_offset) are chosen so that
 // both reads hit every bank once.
 //
 // The scale of K goes into the score.  The scale of V cannot go into the accumulator, which many blocks share, nor into
@@ -26,31 +29,33 @@ namespace fa {
 // Weights of O run up to 2^(kLift + 8 + 1) and so stay in fp16; the lift keeps 2^kLift more of the small ones above its
 // least number.
 constexpr float kLift = 6.f;
+constexpr float kNone = -3e38f;   // a reference of no scores
 
-template <int D>
+template <int D, int NQ>
 struct Paged8Cfg {
   static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
-  static constexpr int kWarps = 4;
-  // What is bound here is the issue of instructions, so as many warps as the registers allow and groups that cost few: us
-  // for 64 sequences, 8 kv heads, at 128 (1K-32K tokens): 16 tokens x 3 CTAs 428, x 4 (spills) 565, 32 x 2 481; at 64
-  // (1K-16K): 16 x 3 179, 32 x 3 162, 32 x 4 147, 64 x 2 173.
-  static constexpr int kStages = D <= 64 ? 2 : D <= 128 ? 4 : 3;
+  static constexpr int kWarps = 4, kRows = 8 * NQ;
+  // Warps as the registers allow without spills, groups as short as the bookkeeping between them allows (us for 64
+  // sequences of 8 kv heads, 8 query rows at most: head 128, 1K-32K tokens 16 tokens x 4 CTAs 355, 32 x 3 355 (one sequence of
+  // 131071: 51, 52), 32 x 2 362; head 64, 1K-16K 32 x 4 115, 16 x 4 124, 16 x 5 118, 64 x 3 121; head 256, 32 sequences of 4 kv
+  // heads 16 x 2 113, x 3 with a stage less 121; 16 rows, head 128, 2 kv heads 16 x 3 102, x 4 (spills) 130, 32 x 3 106).
+  static constexpr int kStages = D <= 64 ? 2 : D > 128 || NQ == 1 ? 3 : 4;
   static constexpr int kTokens = D <= 64 ? 32 : 16;           // tokens of a group
-  static constexpr int kCtas = D <= 64 ? 4 : D <= 128 ? 3 : 2;   // on an SM
+  static constexpr int kCtas = D <= 64 ? 4 : D > 128 ? 2 : 5 - NQ;   // on an SM
   static constexpr int kGroupBytes = kTokens * kD;            // of K or of V
   static constexpr int kStageBytes = 2 * kGroupBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kQBytes = 16 * kD * 2;
+  static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kScales = kQBytes;                     // per warp: of 64 pieces, K and V
   static constexpr int kRowScale = kScales + kWarps * 64 * 8;
-  static constexpr int kStats = kRowScale + 16 * 4;           // per warp and row: maximum, sum, reference of O
-  static constexpr int kRing = (kStats + 3 * kWarps * 16 * 4 + 127) / 128 * 128;
+  static constexpr int kStats = kRowScale + kRows * 4;           // per warp and row: maximum, sum, reference of O
+  static constexpr int kRing = (kStats + 3 * kWarps * kRows * 4 + 127) / 128 * 128;
   static constexpr int kRingBytes = kWarps * kWarpBytes;
-  static constexpr int kMergeBytes = kWarps * 16 * kD * 4;    // fp32 partial outputs, over the ring
+  static constexpr int kMergeBytes = kWarps * kRows * kD * 4;    // fp32 partial outputs, over the ring
   static constexpr int kTotal = kRing + (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes);
 };
 
-// the token, of 8, that column n of a score fragment stands for
+// the token, of 8, that row n of a score fragment stands for
 template <int KD>
 __device__ __forceinline__ constexpr int token_of(int n) {
   const int n0 = n & 1, n1 = n >> 1 & 1, n2 = n >> 2;
@@ -84,17 +89,34 @@ __device__ __forceinline__ void split_scale(float scale, float &exponent, float 
   fraction = e == 255u ? scale : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
 }
 
-// HALF: at most 8 query rows, the upper half of the 16-row tile; the lower half serves the remainder of P.
-template <typename T, int D, typename IdxT, bool HALF>
-__global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas)
+// an 8 x 8 matrix of 16-bit numbers, two of row lane / 4 a lane, into its transpose in the same layout
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float over_tokens_max(float v) {
+#pragma unroll
+  for (int m = 4; m < 32; m *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+  return v;
+}
+__device__ __forceinline__ float over_tokens_sum(float v) {
+#pragma unroll
+  for (int m = 4; m < 32; m *= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+// NQ: columns of 8 query rows
+template <typename T, int D, typename IdxT, int NQ>
+__global__ void __launch_bounds__(Paged8Cfg<D, NQ>::kWarps * 32, Paged8Cfg<D, NQ>::kCtas)
     paged_8bit_kernel(const __grid_constant__ fa_paged_8bit_args p, const Sizing z) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the reduction waits for all of this grid by itself
-  using C = Paged8Cfg<D>;
+  using C = Paged8Cfg<D, NQ>;
   constexpr int KD = C::kD, NW = C::kWarps, NS = C::kStages, GT = C::kTokens;
-  constexpr int R = HALF ? 1 : 2;   // accumulator rows of a thread: g and, in a full tile, g + 8
+  constexpr int R = 2 * NQ;         // query rows of a thread: 2 t4, 2 t4 + 1 of each column
   constexpr int KJ = KD / 64;       // 16-byte pieces of a row that a lane of a quad takes for S
   constexpr int VW = KD / 32;       // 4-byte words of a row that a lane takes for O
-  constexpr int NT = GT / 8, NH = GT / 16;   // score fragments and 16-token pieces of a group
+  constexpr int NH = GT / 16;       // 16-token pieces of a group
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const uint32_t smem = smem_u32(smem_raw);
   const fa_paged_args &a = p.paged;
@@ -142,23 +164,23 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   const int64_t lane_src = (int64_t)lane_r * a.kv_stride_t + ch * 16;
 
   // Where the warp's 16-token pieces lie is worked out for 32 of them at a time, one a lane, and handed on by shuffles: the
-  // table, its bounds and the 64-bit products would otherwise be a sixth of a group's instructions.
+  // table, its bounds and the 64-bit products would otherwise be a sixth of a group's instructions (422 us for 381).
   const auto piece_tok = [&](int q) { return t_begin + (warp + q / NH * NW) * GT + 16 * (q % NH); };
-  IdxT id_ahead = 0;   // of the 32 pieces behind those of `place`
+  int64_t id_ahead = 0;   // of the 32 pieces behind those of `place`
   int64_t place = -1;  // byte offset of this lane's piece; -1: without a token, -2: its id is outside the cache
   const auto look_up = [&](int q0) {
     const int q = q0 + lane, tok = piece_tok(q);
     if (q < my_groups * NH && tok < t_end)
-      id_ahead = static_cast<const IdxT *>(a.block_tables)[(int64_t)seq * a.bt_stride_s + (bs_shift >= 0 ? tok >> bs_shift : tok / BS)];
+      id_ahead = phys_block<IdxT>(a.block_tables, a.bt_stride_s, seq, bs_shift >= 0 ? tok >> bs_shift : tok / BS);
   };
   const auto settle = [&](int q0) {   // the next 32 pieces: their places, their scales into shared memory
     const int q = q0 + lane, tok = piece_tok(q);
     const bool here = q < my_groups * NH && tok < t_end, ok = here && id_ahead >= 0 && id_ahead < p.num_blocks;
     const int in_blk = bs_shift >= 0 ? tok & (BS - 1) : tok % BS;
-    place = ok ? (int64_t)id_ahead * a.kv_stride_b + (int64_t)in_blk * a.kv_stride_t : here ? -2 : -1;
+    place = ok ? id_ahead * a.kv_stride_b + (int64_t)in_blk * a.kv_stride_t : here ? -2 : -1;
     const uint32_t at = scales + (q & 63) * 8;
     if (ok) {
-      const int64_t from = (int64_t)id_ahead * a.num_kv_heads + hk;
+      const int64_t from = id_ahead * a.num_kv_heads + hk;
       cp_async4(at, p.key_scales + from);
       cp_async4(at + 4, p.value_scales + from);
     } else {   // a block outside the cache makes its sequence's output NaN; a piece without tokens counts as nothing
@@ -239,8 +261,8 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   // ---- query group -> shared as fp16 (rows >= `rows` are zero) -----------------
   float *row_scale = reinterpret_cast<float *>(smem_raw + C::kRowScale);
   // threads of a row, and their 8-element pieces; whole warps
-  constexpr int TPR = NW * 2 < KD / 8 ? NW * 2 : KD / 8, PIECES = KD / 8 / TPR;
-  if (tid < 16 * TPR) {
+  constexpr int TPR = NW * 32 / C::kRows < KD / 8 ? NW * 32 / C::kRows : KD / 8, PIECES = KD / 8 / TPR;
+  if (tid < C::kRows * TPR) {
     const int r = tid / TPR, t = tid % TPR;
     const T *q = static_cast<const T *>(a.query) + (int64_t)seq * a.q_stride_s + (int64_t)(qh0 + r) * a.q_stride_h;
     uint4 u[PIECES];
@@ -286,28 +308,33 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
   }
   __syncthreads();
 
-  float q_scale[2];
+  float q_scale[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) q_scale[r] = row_scale[g + 8 * r];
+  for (int r = 0; r < R; ++r) q_scale[r] = row_scale[8 * (r >> 1) + 2 * t4 + (r & 1)];
   // step (j, w) of the contraction is elements 64 j + 16 t4 + 4 w .. + 3 of a row
   constexpr bool kQInRegs = D <= 128;
-  auto q_step = [&](int j, int w, uint32_t (&qa)[4]) {
-    const uint32_t at = smem + (uint32_t)(g * KD + 64 * j + 16 * t4 + 4 * w) * 2;
-    const uint2 x = lds8(at), y = HALF ? make_uint2(0, 0) : lds8(at + 8 * KD * 2);
-    qa[0] = x.x, qa[1] = y.x, qa[2] = x.y, qa[3] = y.y;
+  const auto q_step = [&](int j, int w, int n) {
+    return lds8(smem + (uint32_t)((8 * n + g) * KD + 64 * j + 16 * t4 + 4 * w) * 2);
   };
-  uint32_t qf[kQInRegs ? 4 * KJ : 1][4];
+  uint2 qf[kQInRegs ? 4 * KJ : 1][NQ];
   if (kQInRegs) {
 #pragma unroll
-    for (int i = 0; i < 4 * KJ; ++i) q_step(i / 4, i % 4, qf[i]);
+    for (int i = 0; i < 4 * KJ; ++i)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) qf[i][n] = q_step(i / 4, i % 4, n);
   }
 
-  float acc[KD / 8][4];
+  // acc[m][n]: head elements (lane / 4)'s 2 m and 2 m + 1 of query rows 2 t4, 2 t4 + 1 of column n
+  constexpr int W = VW < 4 ? VW : 4, JV = (VW + 3) / 4;
+  float acc[2 * W * JV][NQ][4];
 #pragma unroll
-  for (int j = 0; j < KD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  float m_i[2] = {-INFINITY, -INFINITY};   // running maximum of the scores
-  float w_i[2] = {-INFINITY, -INFINITY};   // and of score + exponent of V's scale, the reference of acc
-  float l_i[2] = {0.f, 0.f};
+  for (int m = 0; m < 2 * W * JV; ++m)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
+  // references: of the sum, close to the maximum of the scores, and of acc, close to that of score + exponent of V's scale
+  float m_i[R], w_i[R], l_i[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) m_i[r] = w_i[r] = kNone, l_i[r] = 0.f;
 
 #pragma unroll 1
   for (int i = 0; i < my_groups; ++i) {
@@ -318,99 +345,96 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
 
     const int tok0 = t_begin + (warp + i * NW) * GT;
     const uint32_t st = ring + (i % NS) * C::kStageBytes, sv = st + C::kGroupBytes;
-    float ks[NH], ve[NH], vf[NH];
+    const int my_token = token_of<KD>(g);            // of each eight, as a row of S^T
+    const int col[2] = {token_of<KD>(2 * t4), token_of<KD>(2 * t4 + 1)};   // and as a step of O^T
+
+    float s[NH][NQ][4];   // [.][.][2 u + e]: token my_token + 8 u, query row 2 t4 + e
+    float ve[NH], vf[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      const uint2 sc = lds8(scales + (i * NH + h) % 64 * 8);
-      ks[h] = __uint_as_float(sc.x);
-      split_scale(__uint_as_float(sc.y), ve[h], vf[h]);
-    }
-
-    float s[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < NQ; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-      uint4 k[NT];
+      for (int j = 0; j < KJ; ++j) {
+        const uint4 k0 = lds16(st + code_offset<KD>(16 * h + my_token, 4 * j + t4));
+        const uint4 k1 = lds16(st + code_offset<KD>(16 * h + 8 + my_token, 4 * j + t4));
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) k[n] = lds16(st + code_offset<KD>(8 * n + token_of<KD>(g), 4 * j + t4));
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t ka[4] = {codes_lo(w0[w]), codes_lo(w1[w]), codes_hi(w0[w]), codes_hi(w1[w])};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t qa[4];
-        if (!kQInRegs) q_step(j, w, qa);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t kw = w == 0 ? k[n].x : w == 1 ? k[n].y : w == 2 ? k[n].z : k[n].w;
-          Elem<__half>::mma(s[n], kQInRegs ? qf[4 * j + w] : qa, codes_lo(kw), codes_hi(kw));
+          for (int n = 0; n < NQ; ++n) {
+            const uint2 qb = kQInRegs ? qf[4 * j + w][n] : q_step(j, w, n);
+            Elem<__half>::mma(s[h][n], ka, qb.x, qb.y);
+          }
         }
       }
+      const uint2 sc = lds8(scales + (i * NH + h) % 64 * 8);
+      split_scale(__uint_as_float(sc.y), ve[h], vf[h]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float by = q_scale[r] * __uint_as_float(sc.x);
+        s[h][r >> 1][r & 1] *= by, s[h][r >> 1][2 + (r & 1)] *= by;
+      }
     }
-    const bool tail = tok0 + GT > t_end;
-    const int col[2] = {token_of<KD>(2 * t4), token_of<KD>(2 * t4 + 1)};
-    float m_new[2], w_new[2];
+    if (tok0 + GT > t_end) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (tok0 + 16 * h + 8 * u + my_token >= t_end)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) s[h][n][2 * u] = s[h][n][2 * u + 1] = -INFINITY;
+    }
+    // lazy, as in paged.cu: references move when one is 2^8 behind, and only then are lanes' maxima put together
+    float mx[NH][R];
     bool need = false;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float mx[NH];   // of each piece: they have scales of their own
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int h = 0; h < NH; ++h) mx[h] = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float &x = s[n][2 * r + e];
-          x = tail && tok0 + 8 * n + col[e] >= t_end ? -INFINITY : x * (q_scale[r] * ks[n >> 1]);
-          mx[n >> 1] = fmaxf(mx[n >> 1], x);
-        }
-      float most = mx[0], most_w = mx[0] + ve[0];
-      if (NH > 1) most = fmaxf(most, mx[NH - 1]), most_w = fmaxf(most_w, mx[NH - 1] + ve[NH - 1]);
-      m_new[r] = fmaxf(m_i[r], quad_max(most));
-      w_new[r] = fmaxf(w_i[r], quad_max(most_w));
-      // lazy, as in paged.cu: a reference moves when it is 2^8 behind
-      need = need || m_new[r] - m_i[r] > 8.f || w_new[r] - w_i[r] > 8.f;
-    }
+      for (int h = 0; h < NH; ++h) {
+        mx[h][r] = fmaxf(s[h][r >> 1][r & 1], s[h][r >> 1][2 + (r & 1)]);
+        need = need || mx[h][r] - m_i[r] > 8.f || mx[h][r] + (ve[h] - w_i[r]) > 8.f;
+      }
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        l_i[r] *= m_new[r] == -INFINITY ? 1.f : fast_exp2(m_i[r] - m_new[r]);
-        const float alpha = w_new[r] == -INFINITY ? 1.f : fast_exp2(w_i[r] - w_new[r]);
-        m_i[r] = m_new[r], w_i[r] = w_new[r];
+        float m_new = m_i[r], w_new = w_i[r];
 #pragma unroll
-        for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4 / R; ++e) acc[j][2 * r + e] *= alpha;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float m_ref = m_i[r] == -INFINITY ? 0.f : m_i[r];   // all scores -inf: P = 0
-      const float w_ref = w_i[r] == -INFINITY ? 0.f : w_i[r] - kLift;
-      float rs = 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float &x = s[n][2 * r + e];
-          rs += fast_exp2(x - m_ref);
-          x = fast_exp2(x + (ve[n >> 1] - w_ref)) * vf[n >> 1];
+        for (int h = 0; h < NH; ++h) {
+          const float most = over_tokens_max(mx[h][r]);
+          m_new = fmaxf(m_new, most), w_new = fmaxf(w_new, most + ve[h]);
         }
-      l_i[r] += rs;
-    }
-    // P goes in as a 16-bit value and a 16-bit remainder, as in paged.cu
+        l_i[r] *= fast_exp2(m_i[r] - m_new);
+        const float alpha = fast_exp2(w_i[r] - w_new);
+        m_i[r] = m_new, w_i[r] = w_new;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {   // 16 tokens each
-      uint32_t pa[4], pr[4];
-      if (HALF) {
-        split_weights<__half>(s[2 * h][0], s[2 * h][1], pa[0], pa[1]);
-        split_weights<__half>(s[2 * h + 1][0], s[2 * h + 1][1], pa[2], pa[3]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          split_weights<__half>(s[2 * h + (k >> 1)][2 * (k & 1)], s[2 * h + (k >> 1)][2 * (k & 1) + 1], pa[k], pr[k]);
+        for (int m = 0; m < 2 * W * JV; ++m) acc[m][r >> 1][r & 1] *= alpha, acc[m][r >> 1][2 + (r & 1)] *= alpha;
       }
+    }
 #pragma unroll
-      for (int j = 0; j < (VW + 3) / 4; ++j) {
-        constexpr int W = VW < 4 ? VW : 4;
+    for (int h = 0; h < NH; ++h) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float by = ve[h] - w_i[r] + kLift;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float &x = s[h][r >> 1][2 * u + (r & 1)];
+          l_i[r] += fast_exp2(x - m_i[r]);
+          x = fast_exp2(x + by) * vf[h];
+        }
+      }
+      // P goes in as a 16-bit value and a 16-bit remainder, as in paged.cu
+      uint32_t pv[NQ][2], pr[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          split_weights<__half>(s[h][n][2 * u], s[h][n][2 * u + 1], pv[n][u], pr[n][u]);
+          pv[n][u] = transposed(pv[n][u]), pr[n][u] = transposed(pr[n][u]);
+        }
+#pragma unroll
+      for (int j = 0; j < JV; ++j) {
         uint32_t v[4][W];   // tokens 2 t4, 2 t4 + 1 of the first eight and of the second
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -424,65 +448,55 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
           }
         }
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const uint32_t x0 = __byte_perm(v[0][w], v[1][w], 0x5140), x1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-          const uint32_t y0 = __byte_perm(v[2][w], v[3][w], 0x5140), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-          const uint32_t b0[4] = {codes_lo(x0), codes_hi(x0), codes_lo(x1), codes_hi(x1)};
-          const uint32_t b1[4] = {codes_lo(y0), codes_hi(y0), codes_lo(y1), codes_hi(y1)};
+        for (int w = 0; w < W; ++w)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) Elem<__half>::mma(acc[16 * j + 4 * w + e], pa, b0[e], b1[e]);
-          if (!HALF) {
+          for (int e = 0; e < 2; ++e) {
+            const int pick = e ? 0x7362 : 0x5140;
+            const uint32_t x = __byte_perm(v[0][w], v[1][w], pick), y = __byte_perm(v[2][w], v[3][w], pick);
+            const uint32_t va[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) Elem<__half>::mma(acc[16 * j + 4 * w + e], pr, b0[e], b1[e]);
+            for (int n = 0; n < NQ; ++n) {
+              Elem<__half>::mma(acc[2 * (W * j + w) + e][n], va, pv[n][0], pv[n][1]);
+              Elem<__half>::mma(acc[2 * (W * j + w) + e][n], va, pr[n][0], pr[n][1]);
+            }
           }
-        }
       }
     }
     __syncwarp();  // stage may be refilled by the next iteration's issue
   }
   cp_async_wait<0>();
 
-  if (HALF) {
-#pragma unroll
-    for (int j = 0; j < KD / 8; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
-  }
-
   // ---- merge the warps' partial states --------------------------------------
   float *stat_m = reinterpret_cast<float *>(smem_raw + C::kStats);
-  float *stat_l = stat_m + NW * 16, *stat_w = stat_l + NW * 16;
+  float *stat_l = stat_m + NW * C::kRows, *stat_w = stat_l + NW * C::kRows;
   float *merge = reinterpret_cast<float *>(smem_raw + C::kRing);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float l = quad_sum(l_i[r]);
-    if (t4 == 0) {
-      stat_m[warp * 16 + g + 8 * r] = m_i[r];
-      stat_l[warp * 16 + g + 8 * r] = l;
-      stat_w[warp * 16 + g + 8 * r] = w_i[r];
+    const int row = 8 * (r >> 1) + 2 * t4 + (r & 1);
+    const float l = over_tokens_sum(l_i[r]);
+    if (g == 0) {
+      stat_m[warp * C::kRows + row] = m_i[r] == kNone ? -INFINITY : m_i[r];
+      stat_l[warp * C::kRows + row] = l;
+      stat_w[warp * C::kRows + row] = w_i[r] == kNone ? -INFINITY : w_i[r];
     }
   }
   __syncthreads();  // stats visible; every warp has drained its ring
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = g + 8 * r;
+    const int row = 8 * (r >> 1) + 2 * t4 + (r & 1), n = r >> 1, e = r & 1;
     if (row >= rows) continue;
     float ww = -INFINITY;
 #pragma unroll
-    for (int w2 = 0; w2 < NW; ++w2) ww = fmaxf(ww, stat_w[w2 * 16 + row]);
-    const float scale_w = w_i[r] == -INFINITY ? 0.f : fast_exp2(w_i[r] - ww);
-    // a thread's columns 2 t4 and 2 t4 + 1 of the accumulators are two runs of VW words' elements
-    constexpr int W = VW < 4 ? VW : 4;
+    for (int w2 = 0; w2 < NW; ++w2) ww = fmaxf(ww, stat_w[w2 * C::kRows + row]);
+    const float scale_w = w_i[r] == kNone ? 0.f : fast_exp2(w_i[r] - ww);
 #pragma unroll
-    for (int j = 0; j < (VW + 3) / 4; ++j)
+    for (int j = 0; j < JV; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float(&x)[4] = acc[16 * j + 4 * w], (&y)[4] = acc[16 * j + 4 * w + 1];
-          const float(&u)[4] = acc[16 * j + 4 * w + 2], (&v)[4] = acc[16 * j + 4 * w + 3];
-          const int k = 2 * r + e;
-          *reinterpret_cast<float4 *>(merge + (warp * 16 + row) * KD + 128 * j + 4 * W * (2 * t4 + e) + 4 * w) =
-              make_float4(x[k] * scale_w, y[k] * scale_w, u[k] * scale_w, v[k] * scale_w);
-        }
+      for (int w = 0; w < W; ++w) {
+        const float(&x)[4] = acc[2 * (W * j + w)][n], (&y)[4] = acc[2 * (W * j + w) + 1][n];
+        *reinterpret_cast<float4 *>(merge + (warp * C::kRows + row) * KD + 128 * j + 4 * W * g + 4 * w) =
+            make_float4(x[e] * scale_w, x[2 + e] * scale_w, y[e] * scale_w, y[2 + e] * scale_w);
+      }
   }
   __syncthreads();
 
@@ -491,17 +505,17 @@ __global__ void __launch_bounds__(Paged8Cfg<D>::kWarps * 32, Paged8Cfg<D>::kCtas
     float mm = -INFINITY, ww = -INFINITY;
 #pragma unroll
     for (int w2 = 0; w2 < NW; ++w2) {
-      mm = fmaxf(mm, stat_m[w2 * 16 + row]);
-      ww = fmaxf(ww, stat_w[w2 * 16 + row]);
+      mm = fmaxf(mm, stat_m[w2 * C::kRows + row]);
+      ww = fmaxf(ww, stat_w[w2 * C::kRows + row]);
     }
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w2 = 0; w2 < NW; ++w2) {
-      const float mw = stat_m[w2 * 16 + row];
-      if (mw != -INFINITY) l += stat_l[w2 * 16 + row] * fast_exp2(mw - mm);
-      else l += stat_l[w2 * 16 + row];   // 0, or NaN where every score was
-      const float4 v = *reinterpret_cast<const float4 *>(merge + (w2 * 16 + row) * KD + c4 * 4);
+      const float mw = stat_m[w2 * C::kRows + row];
+      if (mw != -INFINITY) l += stat_l[w2 * C::kRows + row] * fast_exp2(mw - mm);
+      else l += stat_l[w2 * C::kRows + row];   // 0, or NaN where every score was
+      const float4 v = *reinterpret_cast<const float4 *>(merge + (w2 * C::kRows + row) * KD + c4 * 4);
       o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
     }
     // from the reference of O to that of the sum; a sequence without tokens has 0, a NaN stays one
@@ -558,11 +572,11 @@ static int validate_8bit(const fa_paged_8bit_args *p) {
   return FA_OK;
 }
 
-template <typename T, int D, typename IdxT, bool HALF>
+template <typename T, int D, typename IdxT, int NQ>
 static int launch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_t stream) {
-  using C = Paged8Cfg<D>;
+  using C = Paged8Cfg<D, NQ>;
   const fa_paged_args *a = &p->paged;
-  auto kern = paged_8bit_kernel<T, D, IdxT, HALF>;
+  auto kern = paged_8bit_kernel<T, D, IdxT, NQ>;
   static unsigned long long attr_done = 0;  // per instantiation, one bit per device
   if (int st = ensure_dyn_smem(kern, C::kTotal, &attr_done)) return st;
   const int q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;
@@ -574,13 +588,13 @@ static int launch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_
 
 template <typename T, typename IdxT>
 static int dispatch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_t s) {
-  const bool half = p->paged.num_q_heads / p->paged.num_kv_heads <= 8;
+  const bool one = p->paged.num_q_heads / p->paged.num_kv_heads <= 8;
   switch (p->paged.head_size) {
-    case 16: return half ? launch_8bit<T, 16, IdxT, true>(p, z, s) : launch_8bit<T, 16, IdxT, false>(p, z, s);
-    case 32: return half ? launch_8bit<T, 32, IdxT, true>(p, z, s) : launch_8bit<T, 32, IdxT, false>(p, z, s);
-    case 64: return half ? launch_8bit<T, 64, IdxT, true>(p, z, s) : launch_8bit<T, 64, IdxT, false>(p, z, s);
-    case 128: return half ? launch_8bit<T, 128, IdxT, true>(p, z, s) : launch_8bit<T, 128, IdxT, false>(p, z, s);
-    default: return half ? launch_8bit<T, 256, IdxT, true>(p, z, s) : launch_8bit<T, 256, IdxT, false>(p, z, s);
+    case 16: return one ? launch_8bit<T, 16, IdxT, 1>(p, z, s) : launch_8bit<T, 16, IdxT, 2>(p, z, s);
+    case 32: return one ? launch_8bit<T, 32, IdxT, 1>(p, z, s) : launch_8bit<T, 32, IdxT, 2>(p, z, s);
+    case 64: return one ? launch_8bit<T, 64, IdxT, 1>(p, z, s) : launch_8bit<T, 64, IdxT, 2>(p, z, s);
+    case 128: return one ? launch_8bit<T, 128, IdxT, 1>(p, z, s) : launch_8bit<T, 128, IdxT, 2>(p, z, s);
+    default: return one ? launch_8bit<T, 256, IdxT, 1>(p, z, s) : launch_8bit<T, 256, IdxT, 2>(p, z, s);
   }
 }
 

@@ -75,16 +75,15 @@ def size_partitions(base, num_seqs, ctas, max_context_len, num_sms, fill=0.8, ma
     pairs = num_seqs * ctas
     if slots and max_context_len < 4096 and (pairs > 2 * num_sms or max_context_len <= 1024):
         # short contexts: four waves of CTAs at most, and partitions that are long where one pass fills the GPU already
-        # (codes of 8 bits, one pass -> this, us: 16 x 1-1000 tokens, 8 kv heads 15.5 -> 12.5, 1 kv head 20 -> 11.6;
-        # 40 x 1-4000, 8 kv heads 74 -> 49, 64 x 4000 133 -> 119, 100 x 1-4000 109 -> 99; contexts far below the bound
-        # pay 3 us)
+        # (codes of 8 bits, one pass -> this, us: 8 kv heads, 16 x 3000 tokens 33 -> 27, 40 x 1-3000 42 -> 32, 64 x 1-3000
+        # 50 -> 46, 100 x 3000 112 -> 104; 1 kv head, 16 x 1-1000 19 -> 11.4; contexts far below the bound pay 3 us)
         size = base if 2 * pairs <= slots * num_sms else 2 * base if pairs <= slots * num_sms else 8 * base
         while size < max_context_len and pairs * _cdiv(max_context_len, size) > 4 * slots * num_sms:
             size *= 2
         return (0, base, base, 0, 1) if max_context_len <= size else (size, size, size, 0, _cdiv(max_context_len, size))
     if 16 * pairs <= slots * num_sms < pairs * _cdiv(max_context_len, base):
-        # few long contexts: one wave of equal partitions, `slots` CTAs an SM (131071 tokens, 8 kv heads, codes of 8 bits: 59
-        # us so, 76 with the power of two below, 71 with the one above)
+        # few long contexts: one wave of equal partitions, `slots` CTAs an SM (131071 tokens, 8 kv heads, codes of 8 bits, an
+        # earlier kernel: 59 us so, 76 with the power of two below, 71 with the one above)
         parts = slots * num_sms // pairs
         finest = size = max(base, _cdiv(_cdiv(max_context_len, parts), 128) * 128)
         while finest % 32 == 0 and finest >= 256:   # for contexts far below the bound
@@ -301,9 +300,9 @@ def _how_8bit(head_size):
     """(fill, many, top, slots) of size_partitions for caches of 8 bits.
 
     A token's bytes are half and a CTA's work on it is not, so partitions end where more CTAs an SM are at hand, and
-    may be longer; the size of a block does not matter.  16-bit rule -> this, us: 37 x 1-8191 tokens, 2 kv heads of 16,
-    head 64 34 -> 25, 64 x 1K-32K, 8 kv heads of 4, head 128 439 -> 422, 2 x 8000 19.6 -> 15, 1 x 30000 in blocks of 256
-    334 -> 22."""
+    may be longer; the size of a block does not matter.  16-bit rule -> this, us (an earlier kernel): 37 x 1-8191 tokens,
+    2 kv heads of 16, head 64 34 -> 25, 64 x 1K-32K, 8 kv heads of 4, head 128 439 -> 422, 2 x 8000 19.6 -> 15, 1 x 30000
+    in blocks of 256 334 -> 22.  One wave of 3 CTAs an SM where 4 fit: one of 131071 51, of 4 56."""
     return 3, 35, 4096, 4 if head_size <= 64 else 3 if head_size <= 128 else 2
 
 
