@@ -20,6 +20,7 @@
 // weights stay in range whatever the scales are (0 too: E = -inf).
 // bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): elements down to 2^-38 of
 // the maximum keep their bits or lose less than 2^-40 of it.
+#include <cfloat>
 #include <climits>
 
 #include "common.cuh"
@@ -29,7 +30,7 @@ namespace fa {
 // Weights of O run up to 2^(kLift + 8 + 1) and so stay in fp16; the lift keeps 2^kLift more of the small ones above its
 // least number.
 constexpr float kLift = 6.f;
-constexpr float kNone = -3e38f;   // a reference of no scores
+constexpr float kNone = -FLT_MAX;   // a reference of no scores: -inf - kNone and kNone - kNone are numbers or -inf
 
 template <int D, int NQ>
 struct Paged8Cfg {

@@ -45,13 +45,13 @@ def call(x, scale, most, splits=0):
     return fa.paged_attention_8bit(q, kc, vc, ks, vs, lens, bt, scale, most, splits)
 
 
-def check(out, x, scale):
+def check(out, x, scale, more=0.0):
     q, kc, vc, ks, vs, lens, bt = x
     want, size, most = cache8.paged_attention_8bit(q, kc, vc, ks, vs, lens, bt, scale)
     half = torch.finfo(q.dtype).eps / 2
     got = out.cpu().double()
     assert out.dtype == q.dtype and torch.isfinite(got).all()
-    bound = half * want.abs() * (1 + half) + (2 * 32 * 2.0 ** -23 * most + 2.0 ** -20 + 2.0 ** -17) * size
+    bound = half * want.abs() * (1 + half) + (2 * 32 * 2.0 ** -23 * most + 2.0 ** -20 + 2.0 ** -17 + more) * size
     off = (got - want).abs() - bound - (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
     assert off.max() <= 0, f"over its bound by {off.max():.3e} of {want.abs().max():.3e}"
 
@@ -190,6 +190,27 @@ def test_a_table_narrower_than_the_lengths():
     assert torch.equal(call(short, 0.125, 100, 1), call(same, 0.125, 100, 1))
     for most, splits in ((100, 2), (100, 0), (9000, 0)):
         check(call(short, 0.125, most, splits), same, 0.125)
+
+
+@pytest.mark.parametrize("D,Hq,BS", [(128, 8, 16), (64, 8, 32), (128, 32, 48), (256, 2, 16), (16, 24, 64)])
+@pytest.mark.parametrize("packed", [True, False])
+def test_one_pass_over_long_sequences(D, Hq, BS, packed):
+    """A warp's places are worked out 32 pieces at a time: around the ends of those, and an id that is wrong behind them.
+
+    One pass: a warp adds its n / 64 pieces up, as value and remainder, in fp32 that the tensor cores may truncate, and
+    their weights, two a piece and lane."""
+    lens = [2047, 2048, 2049, 2064, 4095, 4097, 6150, 1]
+    x = made(lens, Hq, 2, D, BS, torch.float16, seed=D + BS)
+    q, kc, vc, ks, vs, n, bt = (t.cuda() for t in x)
+    if not packed:   # heads inside tokens
+        kc, vc = (c.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(E4M3) for c in (kc, vc))
+    out = fa.paged_attention_8bit(q, kc, vc, ks, vs, n, bt, D ** -0.5, max(lens), 1)
+    check(out, x, D ** -0.5, (2 * max(lens) / 64 + 4) * 2.0 ** -23 + 2 * max(lens) / 64 * 2.0 ** -24)
+    bt[6, 6000 // BS] = kc.shape[0]
+    bt[1, 0] = -5
+    bad = fa.paged_attention_8bit(q, kc, vc, ks, vs, n, bt, D ** -0.5, max(lens), 1)
+    good = [0, 2, 3, 4, 5, 7]
+    assert torch.isnan(bad[[1, 6]]).all() and torch.equal(bad[good], out[good])
 
 
 def test_ids_outside_the_cache_give_nan_and_nothing_else():
