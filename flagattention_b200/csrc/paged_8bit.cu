@@ -36,13 +36,14 @@ template <int D, int NQ>
 struct Paged8Cfg {
   static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
   static constexpr int kWarps = 4, kRows = 8 * NQ;
-  // Warps as the registers allow without spills, groups as short as the bookkeeping between them allows (us for 64
-  // sequences of 8 kv heads, 8 query rows at most: head 128, 1K-32K tokens 16 tokens x 4 CTAs 355, 32 x 3 355 (one sequence of
-  // 131071: 51, 52), 32 x 2 362; head 64, 1K-16K 32 x 4 115, 16 x 4 124, 16 x 5 118, 64 x 3 121; head 256, 32 sequences of 4 kv
-  // heads 16 x 2 113, x 3 with a stage less 121; 16 rows, head 128, 2 kv heads 16 x 3 102, x 4 (spills) 130, 32 x 3 106).
-  static constexpr int kStages = D <= 64 ? 2 : D > 128 || NQ == 1 ? 3 : 4;
-  static constexpr int kTokens = D <= 64 ? 32 : 16;           // tokens of a group
-  static constexpr int kCtas = D <= 64 ? 4 : D > 128 ? 2 : 5 - NQ;   // on an SM
+  // Warps as the registers allow without spills, groups as short as the bookkeeping between them allows.  us for 64
+  // sequences, tokens of a group x CTAs: head 128, 8 kv heads of 4, 1K-32K tokens 16 x 4 355, 32 x 3 355 (one sequence of
+  // 131071: 51, 52), 32 x 2 362, 2 kv heads of 16, 1K-16K 16 x 4 94, 16 x 3 with queries in registers 102, 32 x 3 106; head
+  // 64, 8 kv heads of 4, 1K-16K 32 x 4 115, 16 x 4 124, 16 x 5 118, 64 x 3 121; head 256, 32 sequences of 4 kv heads 16 x 2
+  // 113, x 3 with a stage less 121.
+  static constexpr int kStages = D <= 64 ? 2 : 3;
+  static constexpr int kTokens = D <= 64 ? 32 : 16;     // tokens of a group
+  static constexpr int kCtas = D <= 128 ? 4 : 2;        // on an SM
   static constexpr int kGroupBytes = kTokens * kD;            // of K or of V
   static constexpr int kStageBytes = 2 * kGroupBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D, NQ>::kWarps * 32, Paged8Cfg<D, NQ
 #pragma unroll
   for (int r = 0; r < R; ++r) q_scale[r] = row_scale[8 * (r >> 1) + 2 * t4 + (r & 1)];
   // step (j, w) of the contraction is elements 64 j + 16 t4 + 4 w .. + 3 of a row
-  constexpr bool kQInRegs = D <= 128;
+  constexpr bool kQInRegs = D * NQ <= 128;   // beyond it they would cost a fourth of the warps
   const auto q_step = [&](int j, int w, int n) {
     return lds8(smem + (uint32_t)((8 * n + g) * KD + 64 * j + 16 * t4 + 4 * w) * 2);
   };
