@@ -532,7 +532,7 @@ bool angles_ready(const Tensor &cos, const Tensor &sin, int64_t D, int device) {
     if (!plain(*t, device) || t->scalar_type() != at::kFloat || t->dim() != 2 || !fits(*t) || !vector_ready(*t) ||
         t->requires_grad())
       return false;
-  return cos.sizes() == sin.sizes() && 2 * cos.size(1) <= D && cos.size(1) % 8 == 0;
+  return cos.sizes() == sin.sizes() && cos.numel() > 0 && 2 * cos.size(1) <= D && cos.size(1) % 8 == 0;
 }
 // both weights or neither, of one type
 bool weights_ready(const Tensor &qw, const Tensor &kw, int64_t D, const Tensor &like, int device) {
@@ -639,7 +639,8 @@ variable_list qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &qw,
       !dtype_code(q, &code) || k.scalar_type() != q.scalar_type())
     return {};
   const int64_t B = q.size(0), L = q.size(2), D = q.size(3);
-  if (D % 16 != 0 || D > 512 || k.size(0) != B || k.size(2) != L || k.size(3) != D) return {};
+  if (D % 16 != 0 || D > 512 || D == 0 || k.size(0) != B || k.size(2) != L || k.size(3) != D) return {};
+  if (q.size(1) == 0 || k.size(1) == 0) return {};
   if (!angles_ready(cos, sin, D, device) || !weights_ready(qw, kw, D, q, device)) return {};
   NormCall c{q, k, qw, kw, cos, sin, positions, interleaved, eps};
   if (positions.defined()) {
@@ -665,7 +666,7 @@ variable_list qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &qw,
 
 // a pair of caches with a block table: as the kernels read them, `unit` elements 16 bytes
 bool tables_ready(const Tensor &kc, const Tensor &vc, int64_t Hk, int64_t D, int64_t unit, int device) {
-  if (!plain(kc, device) || !plain(vc, device) || kc.dim() != 4 || kc.sizes() != vc.sizes() || !fits(kc) ||
+  if (!plain(kc, device) || !plain(vc, device) || kc.dim() != 4 || kc.sizes() != vc.sizes() || !fits(kc) || kc.numel() == 0 ||
       kc.strides() != vc.strides() || kc.scalar_type() != vc.scalar_type() || kc.size(1) != Hk || kc.size(3) != D ||
       kc.stride(3) != 1 || !aligned16(kc) || !aligned16(vc))
     return false;
@@ -700,7 +701,7 @@ Tensor rotary_and_cache(const Tensor *const (&t)[9], const Tensor (&o)[6], doubl
     if (!plain(*x, device) || x->dim() != 3 || !fits(*x) || x->scalar_type() != q.scalar_type() || !heads_ready(*x)) return {};
   const int64_t T = q.size(0), D = q.size(2), Hk = k.size(1);
   if (!dtype_code(q, &code) || k.sizes() != v.sizes() || k.size(0) != T || k.size(2) != D) return {};
-  if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return {};
+  if ((D != 16 && D != 32 && D != 64 && D != 128 && D != 256) || q.size(1) == 0) return {};
   const bool held = ks.defined();
   if (held != vs.defined() || !tables_ready(kc, vc, Hk, D, held ? 16 : 8, device) ||
       kc.scalar_type() != (held ? at::kFloat8_e4m3fn : q.scalar_type()))

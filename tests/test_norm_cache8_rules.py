@@ -236,3 +236,28 @@ def test_refusals_on_the_gpu():
                    dict(block_tables=z(1, 3, dtype=torch.int32)), dict(key_scales=torch.ones(6, 3))):
         with pytest.raises(AssertionError):
             write(**change)
+
+
+@pytest.mark.gpu
+def test_calls_without_heads_blocks_or_angles_are_refused():
+    z = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
+    h, c = z(2, 4, 64, dtype=torch.float16), z(6, 4, 16, 64, dtype=torch.float16)
+    lens, bt, ang = z(2, dtype=torch.int32), z(2, 3, dtype=torch.int32), torch.ones(4, 32, device="cuda")
+    fa.rotary_and_cache(h, h, h, c, c.clone(), lens, bt, ang, ang)
+    for args in ((h[:, :0], h, h, c, c, lens, bt, ang, ang), (h, h[:, :0], h[:, :0], c[:, :0], c[:, :0], lens, bt, ang, ang),
+                 (h, h, h, c[:0], c[:0], lens, bt, ang, ang), (h, h, h, c[:, :, :0], c[:, :, :0], lens, bt, ang, ang),
+                 (h, h, h, c, c, lens, bt, ang[:0], ang[:0]), (h, h, h, c, c, lens, bt, ang[:, :0], ang[:, :0])):
+        with pytest.raises(AssertionError):
+            fa.rotary_and_cache(*args)
+    q = z(2, 4, 3, 64, dtype=torch.float16)
+    for args in ((q[:, :0], q, None, None, ang, ang), (q, q[:, :0], None, None, ang, ang),
+                 (q, q, None, None, ang[:0], ang[:0]), (q, q, None, None, ang[:, :0], ang[:, :0]),
+                 (q[..., :0], q[..., :0], None, None, ang[:, :0], ang[:, :0])):
+        with pytest.raises(AssertionError):
+            fa.qk_norm_rotary(*args)
+    e = z(6, 2, 16, 64, dtype=E4M3)
+    s = z(6, 2)
+    for args in ((h[:, :0], e, e, s, s), (h, e[:, :0], e[:, :0], s[:, :0], s[:, :0]), (h, e[:0], e[:0], s[:0], s[:0]),
+                 (h, e[:, :, :0], e[:, :, :0], s, s)):
+        with pytest.raises(AssertionError):
+            fa.paged_attention_8bit(*args, lens, bt, 0.1, 48)
