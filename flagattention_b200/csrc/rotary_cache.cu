@@ -30,6 +30,9 @@ namespace fa {
 constexpr int kCacheThreads = 128;
 constexpr int kTile = 32;     // rows whose units a CTA of the 8-bit part finds at once, one a lane
 constexpr int kAhead = 4;     // heads of a row whose loads are in flight
+// passes over a unit whose values wait for its scale in shared memory, 8 KB each (blocks of 64 tokens, head 128, 5800 rows of
+// prompts: 66 us, worked out twice 81)
+constexpr int kKept = 3;
 
 struct RotaryCache {
   fa_rotary_cache_args p;
@@ -367,10 +370,10 @@ __device__ __forceinline__ void move_codes(uint8_t *dst, int64_t stride, int row
 }
 
 // The units of a block's heads [h_lo, h_hi), one after another: the next head's loads are in flight, and the rows' angles
-// stay in registers.
+// stay in registers.  `kept` has room for the values of kKept passes.
 template <typename T, int LPR, bool IL, int TEAM>
 __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq, int place,
-                                         int left, int h_lo, int h_hi, bool key, uint32_t *shared_most) {
+                                         int left, int h_lo, int h_hi, bool key, uint32_t *shared_most, float4 *kept) {
   constexpr int kWarps = TEAM / 32;
   const int off = place % p.block_size;
   const Unit<T, LPR, IL, TEAM> u{p, lane, row, place, min(left, p.block_size - off), key};
@@ -387,14 +390,15 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
   for (int h = h_lo; h < h_hi; ++h) {
     const float old = off ? scales[h] : 0.f;   // a block's first token: what the block held before is over
     uint8_t *cache = caches + h * p.kv_stride_h, *dst = cache + off * p.kv_stride_t;
-    // The values' maximum, in one step for each pass; then their codes, from what one pass left in the registers, or by
-    // the same steps once more.
-    const int steps = passes == 1 ? 1 : 2 * passes;
+    // The values' maximum, in one step for each pass; then their codes: of the last pass from registers, of the first
+    // ones as they were kept (by the thread that needs them again), of those between by the same steps once more.
+    const int steps = passes + max(passes - 1 - kKept, 0);
+    const auto pass_of = [&](int step) { return step < passes ? step : step - passes + kKept; };
     uint32_t most = 0;
     float now = 0.f;
 #pragma unroll 1
     for (int step = 0; step < steps; ++step) {
-      const int pass = step < passes ? step : step - passes, next = pass + 1 < passes ? pass + 1 : 0;
+      const int pass = pass_of(step), next = step + 1 < steps ? pass_of(step + 1) : 0;
       u.values(x, c, s, lo, hi);
       // what the next step works on, under the rest of this one
       if (step + 1 < steps || h + 1 < h_hi) {
@@ -402,6 +406,11 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
         if (passes > 1) u.angles(next, c, s);
       }
       if (step < passes) most = max(most, u.largest(pass, lo, hi));
+      if (step < kKept && step + 1 < passes) {
+        float4 *at = kept + step * 4 * TEAM + u.thread();
+        at[0] = make_float4(lo[0], lo[1], lo[2], lo[3]), at[TEAM] = make_float4(lo[4], lo[5], lo[6], lo[7]);
+        at[2 * TEAM] = make_float4(hi[0], hi[1], hi[2], hi[3]), at[3 * TEAM] = make_float4(hi[4], hi[5], hi[6], hi[7]);
+      }
       if (step == passes - 1) {
         most = __reduce_max_sync(0xffffffffu, most);
         if (kWarps > 1) {   // the team's
@@ -416,8 +425,20 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
         if (off && now > old)
           move_codes(cache, p.kv_stride_t, off, p.head_size, (double)old / (double)now, u.thread(), TEAM);
       }
-      if (passes == 1 || step >= passes)
+      if (step >= passes - 1) u.store(pass, lo, hi, now, dst);
+    }
+    if (kWarps > 1) {
+#pragma unroll 1
+      for (int pass = 0; pass < min(kKept, passes - 1); ++pass) {
+        const float4 *at = kept + pass * 4 * TEAM + u.thread();
+        const float4 v[4] = {at[0], at[TEAM], at[2 * TEAM], at[3 * TEAM]};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          lo[4 * k] = v[k].x, lo[4 * k + 1] = v[k].y, lo[4 * k + 2] = v[k].z, lo[4 * k + 3] = v[k].w;
+          hi[4 * k] = v[2 + k].x, hi[4 * k + 1] = v[2 + k].y, hi[4 * k + 2] = v[2 + k].z, hi[4 * k + 3] = v[2 + k].w;
+        }
         u.store(pass, lo, hi, now, dst);
+      }
     }
     if (u.thread() == 0) scales[h] = now;
   }
@@ -434,10 +455,12 @@ __device__ __forceinline__ void unit_part(const RotaryCache &a) {
     if (row >= p.num_tokens) return;
     const Token t = find_token(p, row);
     if (t.valid)
-      units_of<T, LPR, IL, 32>(p, lane, row, t.seq, t.place, 1, rest / 2, rest / 2 + 1, rest % 2 == 0, nullptr);
+      units_of<T, LPR, IL, 32>(p, lane, row, t.seq, t.place, 1, rest / 2, rest / 2 + 1, rest % 2 == 0, nullptr,
+                                   nullptr);
     return;
   }
   __shared__ uint32_t shared_most[2 * kCacheThreads / 32];
+  __shared__ float4 kept[kKept * 4 * kCacheThreads];
   const int tile = blockIdx.x / a.unit_ctas_y, y = blockIdx.x % a.unit_ctas_y;
   const Token t = find_token(p, tile * kTile + lane_id);
   const bool leads = t.valid && (t.first || t.place == 0 || t.place % p.block_size == 0);
@@ -449,7 +472,7 @@ __device__ __forceinline__ void unit_part(const RotaryCache &a) {
     const int from = __fns(several, 0, i / per_block + 1), rest = i % per_block, h = rest / 2 * a.unit_heads;
     units_of<T, LPR, IL, kCacheThreads>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from),
                                         from_lane(t.left, from), h, min(h + a.unit_heads, p.num_kv_heads), rest % 2 == 0,
-                                        shared_most);
+                                        shared_most, kept);
     __syncthreads();   // shared_most is the next one's
   }
   // single tokens: a warp for each and head
@@ -457,7 +480,7 @@ __device__ __forceinline__ void unit_part(const RotaryCache &a) {
   for (int i = y * (kCacheThreads / 32) + warp; i < ones; i += a.unit_ctas_y * (kCacheThreads / 32)) {
     const int from = __fns(single, 0, i / per_row + 1), rest = i % per_row;
     units_of<T, LPR, IL, 32>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from), 1, rest / 2,
-                             rest / 2 + 1, rest % 2 == 0, nullptr);
+                             rest / 2 + 1, rest % 2 == 0, nullptr, nullptr);
   }
 }
 
