@@ -57,12 +57,12 @@ __device__ __forceinline__ void load_weight8(float (&w)[8], const void *weight, 
 template <typename T, int LPR, bool IL>
 struct NormLane {
   int off_a, off_b, b, l, h_lo, h_hi, e;   // e: 0 q, 1 k
-  bool live;
+  bool live, turns;
   float c[8], s[8], wlo[8], whi[8];
 
   __device__ __forceinline__ void columns(const NormArgs &a) {
     const int j = threadIdx.x % LPR;
-    const bool turns = j < a.R / 16;
+    turns = j < a.R / 16;
     off_a = IL || !turns ? 16 * j : 8 * j;
     off_b = IL || !turns ? 16 * j + 8 : a.R / 2 + 8 * j;
     live = j < a.D / 16;
@@ -91,15 +91,14 @@ struct NormLane {
   // the position of row `row` of the batch element, and its angles
   __device__ __forceinline__ void turn_to(const NormArgs &a, int row) {
     l = row;
-    const int j = threadIdx.x % LPR;
     const bool here = live && l < a.L;
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-    if (here && j < a.R / 16) {
+    if (here && turns) {
       int64_t pos = a.positions ? a.positions[b * a.pos_stride_b + l] : l;
       // a position outside the tables reads the nearest row instead of foreign memory
       pos = pos < 0 ? 0 : (pos >= a.table_rows ? a.table_rows - 1 : pos);
-      const int64_t at = pos * (a.R / 2) + 8 * j;
+      const int64_t at = pos * (a.R / 2) + 8 * (threadIdx.x % LPR);
       load8(c, a.cos + at);
       load8(s, a.sin + at);
     }
@@ -159,8 +158,9 @@ __global__ void __launch_bounds__(kNormThreads, kForwardCtas) qk_norm_rotary_fwd
       to_pairs<IL>(lo, hi, va, vb);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ylo[i] = (lo[i] * ll[i] - hi[i] * lh[i]) * r;
-        yhi[i] = (hi[i] * hh[i] + lo[i] * hl[i]) * r;
+        // (elements that only pass have no partner: 0 times an infinity would be NaN)
+        ylo[i] = (lo[i] * ll[i] - (t.turns ? hi[i] : 0.f) * lh[i]) * r;
+        yhi[i] = (hi[i] * hh[i] + (t.turns ? lo[i] : 0.f) * hl[i]) * r;
       }
       from_pairs<IL>(va, vb, ylo, yhi);
       if (here) {
@@ -266,7 +266,9 @@ __global__ void __launch_bounds__(kNormThreads, kBackwardCtas) qk_norm_rotary_bw
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             ss = fmaf(xlo[i], xlo[i], fmaf(xhi[i], xhi[i], ss));
-            const float hl = glo[i] * t.c[i] + ghi[i] * t.s[i], hh = ghi[i] * t.c[i] - glo[i] * t.s[i];
+            // (elements that only pass have no partner: 0 times an infinity would be NaN)
+            const float hl = t.turns ? glo[i] * t.c[i] + ghi[i] * t.s[i] : glo[i];
+            const float hh = t.turns ? ghi[i] * t.c[i] - glo[i] * t.s[i] : ghi[i];
             tlo[i] = hl * xlo[i], thi[i] = hh * xhi[i];
             ax = fmaf(tlo[i], t.wlo[i], fmaf(thi[i], t.whi[i], ax));
             glo[i] = hl * t.wlo[i], ghi[i] = hh * t.whi[i];

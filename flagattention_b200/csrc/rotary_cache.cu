@@ -227,8 +227,9 @@ __device__ __forceinline__ void row_part(const RotaryCache &a) {
       to_pairs<IL>(lo, hi, va, vb);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ylo[i] = (lo[i] * ll[i] - hi[i] * lh[i]) * r;
-        yhi[i] = (hi[i] * hh[i] + lo[i] * hl[i]) * r;
+        // (elements that only pass have no partner: 0 times an infinity would be NaN)
+        ylo[i] = (lo[i] * ll[i] - (lane.turns ? hi[i] : 0.f) * lh[i]) * r;
+        yhi[i] = (hi[i] * hh[i] + (lane.turns ? lo[i] : 0.f) * hl[i]) * r;
       }
       from_pairs<IL>(va, vb, ylo, yhi);
       ua[u] = pack8<T>(va), ub[u] = pack8<T>(vb);
@@ -308,12 +309,17 @@ struct Unit {
       r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + (double)p.eps);
       lane.template weights<T>(p, p.k_weight, wlo, whi);
     }
+    if (lane.turns) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      double l = lo[k], h = hi[k];
-      if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
-      lo[k] = to_odd(l * c[k] - h * s[k]);
-      hi[k] = to_odd(h * c[k] + l * s[k]);
+      for (int k = 0; k < 8; ++k) {
+        double l = lo[k], h = hi[k];
+        if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
+        lo[k] = to_odd(l * c[k] - h * s[k]);
+        hi[k] = to_odd(h * c[k] + l * s[k]);
+      }
+    } else if (p.k_weight) {   // elements that only pass have no partner: 0 times an infinity would be NaN
+#pragma unroll
+      for (int k = 0; k < 8; ++k) lo[k] = to_odd(lo[k] * (r * wlo[k])), hi[k] = to_odd(hi[k] * (r * whi[k]));
     }
   }
   __device__ __forceinline__ uint32_t largest(int pass, const float (&lo)[8], const float (&hi)[8]) const {

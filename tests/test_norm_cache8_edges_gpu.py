@@ -1,0 +1,96 @@
+"""Corners of qk_norm_rotary, rotary_and_cache and paged_attention_8bit, against their definitions in 64 bits: infinities beside
+elements that only pass, batches cut short, scales that are no powers of two, the smallest scales, eps of 0."""
+import pytest
+import torch
+
+import flagattention_b200 as fa
+from oracle import cache8
+from test_rotary_cache_gpu import E4M3, Batch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def same_where_not_finite(got, want):
+    """NaN where the definition has NaN, infinities where it has those; returns where both are finite."""
+    got, want = got.detach().cpu().double(), want.double()
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), finite)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[got.isinf()], want[want.isinf()])
+    return finite
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("held", [True, False])
+@pytest.mark.parametrize("norm", [None, "fp32"])
+@pytest.mark.parametrize("R", [32, 64])
+def test_an_infinity_stays_among_the_elements_that_only_pass(R, norm, held, interleaved):
+    """Partial rotation: an element behind the rotated ones has no partner, so an infinity or a NaN in it is its own affair.  With
+    the norm its row's r is 0 (NaN) instead, for either form.
+
+    Queries and 16-bit keys: half a step and the 64 roundings of test_rotary_cache_gpu.py, of the sizes of finite terms."""
+    D = 128
+    b = Batch([3, 0, 20], [18, 1, 5], 2, 2, D, 16, torch.bfloat16, held, R=R, norm=norm, seed=R, interleaved=interleaved)
+    q, k, _ = b.parts(b.qkv)
+    inf, nan = float("inf"), float("nan")
+    for x in (q, k):
+        x[1, 0, R + 3], x[2, 1, R], x[4, 0, D - 1], x[5, 1, R + 17] = inf, -inf, inf, nan
+        x[18, 0, R + 8:R + 12] = inf
+        x[20, 1, 5] = inf       # among the rotated ones: its pair
+    d = b.device()
+    out = b.call(d)
+    want_q, kc, vc, ks, vs = b.expected()
+    pairs = [(out, want_q)]
+    if held:
+        assert torch.equal(d["ks"].cpu().double(), ks) and torch.equal(d["vs"].cpu().double(), vs)
+        got = d["kc"].cpu().view(E4M3).double()
+        assert ((got == kc) | (got.isnan() & kc.isnan())).all()
+    else:
+        assert torch.equal(d["vc"].cpu().double(), vc)
+        pairs.append((d["kc"], kc))
+    b.qkv = torch.where(torch.isfinite(b.qkv), b.qkv, 0.0)
+    sizes = b.expected(abs_=True)
+    for (got, want), size in zip(pairs, sizes):
+        ok = same_where_not_finite(got, want)
+        if norm:   # (rows with an infinity or a NaN have r of 0 or NaN; the sizes are those of the row without it)
+            assert ok.any()
+        off = (got.cpu().double() - want).abs() - 2.0 ** -8 * want.abs() * (1 + 2.0 ** -8) - 64 * U * size
+        assert off[ok].max() <= 0
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("weights", [True, False])
+def test_an_infinity_stays_in_its_element_of_norm_and_gradients(weights, interleaved):
+    """The same of qk_norm_rotary: with an infinity in a row r is 0, and only the infinite element is NaN.  In the gradient of the
+    result an infinity reaches its own column of the weight's gradient and no other."""
+    B, H, L, D, R = 2, 3, 21, 96, 32
+    gen = torch.Generator().manual_seed(1)
+    x, g = (torch.randn(B, H, L, D, generator=gen).to(torch.bfloat16) for _ in range(2))
+    w = 1 + 0.3 * torch.randn(D, generator=gen) if weights else None
+    cos, sin = fa.rotary_tables(L, R)
+    x[0, 1, 4, R + 5] = float("inf")
+    x[1, 2, 20, D - 1] = -float("inf")
+    x[1, 0, 3, R + 9] = float("nan")
+    c = {n: None if t is None else t.cuda() for n, t in dict(x=x, w=w, cos=cos, sin=sin).items()}
+    y, _ = fa.qk_norm_rotary(c["x"], c["x"], c["w"], c["w"], c["cos"], c["sin"], interleaved=interleaved)
+    want = cache8.norm_rotary(x, w, cos, sin, None, interleaved)
+    ok = same_where_not_finite(y, want)
+    assert ok[0, 1, 4].sum() == D - 1 and ok[1, 2, 20].sum() == D - 1 and not ok[1, 0, 3].any()
+    clean = torch.where(torch.isfinite(x), x, 0.0).abs()
+    size = torch.maximum(*(cache8.norm_rotary(clean, None if w is None else w.abs(), cos.abs(), s, None, interleaved).abs()
+                           for s in (sin.abs(), -sin.abs())))
+    off = (y.cpu().double() - want).abs() - 2.0 ** -8 * want.abs() * (1 + 2.0 ** -8) - 64 * U * size
+    assert off[ok].max() <= 0
+    if w is None:
+        return
+    x = clean.float().to(torch.bfloat16) + 0.5
+    g[1, 1, 7, R + 11] = float("inf")
+    g[0, 0, 20, D - 8] = -float("inf")
+    xs, ws = x.cuda().requires_grad_(), c["w"].requires_grad_()
+    y, _ = fa.qk_norm_rotary(xs, xs.detach(), ws, c["w"].detach(), c["cos"], c["sin"], interleaved=interleaved)
+    dw, = torch.autograd.grad(y, ws, g.cuda())
+    _, want, _, size = cache8.norm_rotary_backward(x, w, torch.where(torch.isfinite(g), g, 0.0), cos, sin, None, interleaved)
+    reached = torch.zeros(D, dtype=torch.bool)
+    reached[[R + 11, D - 8]] = True
+    assert torch.equal(dw.cpu().isfinite(), ~reached)
+    assert ((dw.cpu().double() - want).abs() - 2.0 ** -24 * want.abs() - 256 * U * size)[~reached].max() <= 0
