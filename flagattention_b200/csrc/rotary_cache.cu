@@ -55,6 +55,7 @@ struct Token {
 // Called by whole warps; every lane has a row of its own (row >= num_tokens: none).
 __device__ __forceinline__ Token find_token(const fa_rotary_cache_args &p, int row) {
   Token t{row, 0, 1, true, false};
+  int to_end = 1;   // `left`, and those tokens of its sequence that the call has no rows for
   if (p.query_starts) {
     // the last start that is not behind the row, 32 starts at a time: their loads do not depend on one another
     int before = 0;
@@ -70,14 +71,15 @@ __device__ __forceinline__ Token find_token(const fa_rotary_cache_args &p, int r
     }
     t.seq = before - 1;
     if (t.seq < 0 || t.seq >= p.num_seqs || row >= p.num_tokens) return t;
-    t.left = min(p.query_starts[t.seq + 1], p.num_tokens) - row;
+    const int end = p.query_starts[t.seq + 1];
+    to_end = end - row, t.left = min(end, p.num_tokens) - row;
     t.first = row == p.query_starts[t.seq];
   } else if (row >= p.num_tokens) {
     return t;
   }
   const int len = p.context_lens[t.seq];
-  if (t.left > len) return t;   // in front of its sequence
-  t.place = len - t.left;
+  if (to_end > len) return t;   // in front of its sequence
+  t.place = len - to_end;
   t.valid = t.left > 0 && t.place / p.block_size < p.table_cols;
   return t;
 }

@@ -383,8 +383,8 @@ def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, bl
 
     query [num_tokens, heads, head], key, value [num_tokens, kv_heads, head], fp16 / bf16, head 16, 32, 64, 128 or 256.
     context_lens [num_seqs] counts the new tokens, as the attention that follows takes it; sequence s has rows
-    query_starts[s] .. query_starts[s + 1] - 1 (integers [num_seqs + 1], ascending), the last of them its last token; None: one
-    row a sequence.  block_tables [num_seqs, max_blocks].  A row's position in the tables is its place in its sequence,
+    query_starts[s] .. query_starts[s + 1] - 1 (integers [num_seqs + 1], ascending), the last of them its last token (those from
+    num_tokens on are not there); None: one row a sequence.  block_tables [num_seqs, max_blocks].  A row's position in the tables is its place in its sequence,
     or positions [num_tokens], clamped to them.  cos, sin, weights, eps, interleaved: as in qk_norm_rotary, no norm
     without weights.
 

@@ -437,7 +437,7 @@ int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, con
  * and rotated as above, queries go to `out`, keys and values to their places.
  *   Sequence s has the rows [query_starts[s], query_starts[s + 1]) (NULL: row s alone, num_tokens == num_seqs), the
  * last of which is token context_lens[s] - 1 of the sequence: lengths count the new tokens, as the attention that
- * follows wants them.  A token's place is position place % block_size of block block_tables[s, place / block_size],
+ * follows wants them.  Rows from num_tokens on are not there, and those in front of them stay where they are.  A token's place is position place % block_size of block block_tables[s, place / block_size],
  * its angle's row positions[row] or its place.  Rows of no sequence, rows in front of their sequence (more
  * rows than tokens) and rows behind the table's columns are written nowhere and have 0 in `out`; a block id outside
  * [0, num_blocks) is not written to.  A block that is written to belongs to one sequence.

@@ -94,3 +94,18 @@ def test_an_infinity_stays_in_its_element_of_norm_and_gradients(weights, interle
     reached[[R + 11, D - 8]] = True
     assert torch.equal(dw.cpu().isfinite(), ~reached)
     assert ((dw.cpu().double() - want).abs() - 2.0 ** -24 * want.abs() - 256 * U * size)[~reached].max() <= 0
+
+
+@pytest.mark.parametrize("held", [True, False])
+def test_starts_that_reach_beyond_the_rows(held):
+    """A batch cut short, or static starts: a row's place goes by the starts and not by the rows that are there."""
+    for keep in (31, 17, 16, 3, 1):
+        b = Batch([5, 0, 40], [20, 9, 30], 4, 2, 64, 16, torch.bfloat16, held, seed=keep)
+        b.qkv = b.qkv[:keep]
+        d = b.device()
+        b.check(b.call(d), d)
+    # single rows, and a sequence whose other rows are all missing
+    b = Batch([15, 7, 3], [1, 1, 12], 4, 2, 64, 16, torch.float16, held, seed=1)
+    b.qkv = b.qkv[:3]
+    d = b.device()
+    b.check(b.call(d), d)
