@@ -11,7 +11,8 @@
 // relative step at every exponent), and when a later token needs a larger one the old codes only move in exponent: exact
 // but below 2^-6 of the new scale, where e4m3 loses bits.  A block filled token by token is the block filled at once.
 // An e4m3 code jumps at its borders, and so does a scale: a key is worked out in 64 bits and taken to fp32 by rounding to odd
-// (truncated, the last bit set if anything was lost), which keeps comparisons and the second rounding right.  (fp32 with a
+// (truncated, the last bit set if anything was lost), which keeps comparisons and the second rounding right under a scale that is
+// a power of two (another one, in a cache that was not filled here: divide_units()).  (fp32 with a
 // known error and 64 bits only where that leaves two codes: slower, 7.3 us for 4.5 at 64 single tokens, 53 for 44 at 5800
 // rows of prompts.  Some warp always has such an element, and the second way costs the first one its registers.)
 
@@ -20,6 +21,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "flagattn_b200.h"
@@ -268,6 +270,35 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
+// A key's pairs (lo, hi) normed and rotated in 64 bits: f(k, lo[k], hi[k]).  Whole warps.
+template <typename T, int LPR, bool IL, typename F>
+__device__ __forceinline__ void key_pairs(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, const float (&c)[8],
+                                          const float (&s)[8], const float (&lo)[8], const float (&hi)[8], F f) {
+  float wlo[8], whi[8];
+  double r = 1.0;
+  if (p.k_weight) {
+    double ss = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss += (double)lo[k] * lo[k] + (double)hi[k] * hi[k];
+    r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + (double)p.eps);
+    lane.template weights<T>(p, p.k_weight, wlo, whi);
+  }
+  if (lane.turns) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      double l = lo[k], h = hi[k];
+      if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
+      f(k, l * c[k] - h * s[k], h * c[k] + l * s[k]);
+    }
+  } else if (p.k_weight) {   // elements that only pass have no partner: 0 times an infinity would be NaN
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f(k, lo[k] * (r * wlo[k]), hi[k] * (r * whi[k]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f(k, (double)lo[k], (double)hi[k]);
+  }
+}
+
 // The threads that work on a unit, TEAM of them, and the row of a pass that each has a part of.
 template <typename T, int LPR, bool IL, int TEAM>
 struct Unit {
@@ -280,12 +311,15 @@ struct Unit {
   static __device__ __forceinline__ int thread() { return threadIdx.x % TEAM; }
   static __device__ __forceinline__ int row_of(int pass) { return pass * kRowsPass + thread() / LPR; }
 
+  __device__ __forceinline__ const T *source(int i, int head) const {
+    return key ? static_cast<const T *>(p.key) + (row0 + i) * p.k_stride_t + head * p.k_stride_h
+               : static_cast<const T *>(p.value) + (row0 + i) * p.v_stride_t + head * p.v_stride_h;
+  }
   __device__ __forceinline__ void load(int pass, int head, uint4 (&u)[2]) const {
     const int i = row_of(pass);
     u[0] = u[1] = make_uint4(0, 0, 0, 0);
     if (i < n) {
-      const T *src = key ? static_cast<const T *>(p.key) + (row0 + i) * p.k_stride_t + head * p.k_stride_h
-                         : static_cast<const T *>(p.value) + (row0 + i) * p.v_stride_t + head * p.v_stride_h;
+      const T *src = source(i, head);
       u[0] = read16(src + lane.off_a);
       u[1] = read16(src + lane.off_b);
     }
@@ -301,28 +335,8 @@ struct Unit {
     unpack8<T>(va, u[0]);
     unpack8<T>(vb, u[1]);
     to_pairs<IL>(lo, hi, va, vb);
-    if (!key) return;
-    float wlo[8], whi[8];
-    double r = 1.0;
-    if (p.k_weight) {
-      double ss = 0.0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) ss += (double)va[k] * va[k] + (double)vb[k] * vb[k];
-      r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + (double)p.eps);
-      lane.template weights<T>(p, p.k_weight, wlo, whi);
-    }
-    if (lane.turns) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        double l = lo[k], h = hi[k];
-        if (p.k_weight) l *= r * wlo[k], h *= r * whi[k];
-        lo[k] = to_odd(l * c[k] - h * s[k]);
-        hi[k] = to_odd(h * c[k] + l * s[k]);
-      }
-    } else if (p.k_weight) {   // elements that only pass have no partner: 0 times an infinity would be NaN
-#pragma unroll
-      for (int k = 0; k < 8; ++k) lo[k] = to_odd(lo[k] * (r * wlo[k])), hi[k] = to_odd(hi[k] * (r * whi[k]));
-    }
+    if (key)
+      key_pairs<T>(p, lane, c, s, lo, hi, [&](int k, double l, double h) { lo[k] = to_odd(l), hi[k] = to_odd(h); });
   }
   __device__ __forceinline__ uint32_t largest(int pass, const float (&lo)[8], const float (&hi)[8]) const {
     float most = 0.f;   // an infinity saturates, a NaN stays one (a maximum passes over it): no scale holds them
@@ -342,16 +356,10 @@ struct Unit {
                                         uint8_t *dst) const {
     const int i = row_of(pass);
     if (i >= n) return;
+    const float inv = 1.f / scale;   // (products with it are exact)
     float x[8], y[8], a[8], b[8];
-    if ((__float_as_uint(scale) & 0x7fffffu) == 0) {   // a power of two, as this kernel leaves them: products are exact
-      const float inv = 1.f / scale;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = lo[k] * inv, y[k] = hi[k] * inv;
-    } else {
-      const double inv = 1.0 / (double)scale;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = to_odd((double)lo[k] * inv), y[k] = to_odd((double)hi[k] * inv);
-    }
+    for (int k = 0; k < 8; ++k) x[k] = lo[k] * inv, y[k] = hi[k] * inv;
     from_pairs<IL>(a, b, x, y);
     uint8_t *at = dst + i * p.kv_stride_t;
     *reinterpret_cast<uint2 *>(at + lane.off_a) =
@@ -380,9 +388,10 @@ __device__ __forceinline__ void move_codes(uint8_t *dst, int64_t stride, int row
 }
 
 // The units of a block's heads [h_lo, h_hi), one after another: the next head's loads are in flight, and the rows' angles
-// stay in registers.  `kept` has room for the values of kKept passes.
+// stay in registers.  `kept` has room for the values of kKept passes.  Returns the mantissas of their scales, 0 where those are
+// powers of two.
 template <typename T, int LPR, bool IL, int TEAM>
-__device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq, int place,
+__device__ __forceinline__ uint32_t units_of(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq, int place,
                                          int left, int h_lo, int h_hi, bool key, uint32_t *shared_most, float4 *kept) {
   constexpr int kWarps = TEAM / 32;
   const int off = place % p.block_size;
@@ -393,9 +402,10 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
   u.load(0, h_lo, x);
   u.angles(0, c, s);
   const int64_t blk = block_of(p, seq, place / p.block_size);
-  if (blk < 0) return;   // (the same for the whole team)
+  if (blk < 0) return 0;   // (the same for the whole team)
   float *scales = (key ? p.key_scales : p.value_scales) + blk * p.num_kv_heads;
   uint8_t *caches = static_cast<uint8_t *>(key ? p.key_cache : p.value_cache) + blk * p.kv_stride_b;
+  uint32_t mantissas = 0;
 #pragma unroll 1
   for (int h = h_lo; h < h_hi; ++h) {
     const float old = off ? scales[h] : 0.f;   // a block's first token: what the block held before is over
@@ -432,6 +442,7 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
         }
         now = scale_for(most);
         now = fmaxf(old, now);
+        mantissas |= __float_as_uint(now) & 0x7fffffu;
         if (off && now > old)
           move_codes(cache, p.kv_stride_t, off, p.head_size, (double)old / (double)now, u.thread(), TEAM);
       }
@@ -452,25 +463,61 @@ __device__ __forceinline__ void units_of(const fa_rotary_cache_args &p, const La
     }
     if (u.thread() == 0) scales[h] = now;
   }
+  return mantissas;
 }
 
-template <typename T, int LPR, bool IL, bool ONE>
-__device__ __forceinline__ void unit_part(const RotaryCache &a) {
+// The codes of those heads whose scale is no power of two, which only a cache that someone else filled has, once more from
+// the operands.  A border between two codes times such a scale has up to 29 bits, so neither the 24 bits of a key tell on
+// which side of it the key is, nor does a product with the scale's reciprocal.
+template <typename T, int LPR, bool IL, int TEAM>
+__device__ __forceinline__ void divide_units(const fa_rotary_cache_args &p, const Lane<LPR, IL> &lane, int row, int seq,
+                                             int place, int left, int h_lo, int h_hi, bool key) {
+  const int off = place % p.block_size;
+  const Unit<T, LPR, IL, TEAM> u{p, lane, row, place, min(left, p.block_size - off), key};
+  const int64_t blk = block_of(p, seq, place / p.block_size);
+  if (blk < 0) return;
+  const float *scales = (key ? p.key_scales : p.value_scales) + blk * p.num_kv_heads;
+  uint8_t *caches = static_cast<uint8_t *>(key ? p.key_cache : p.value_cache) + blk * p.kv_stride_b;
+#pragma unroll 1
+  for (int h = h_lo; h < h_hi; ++h) {
+    const float scale = scales[h];
+    if ((__float_as_uint(scale) & 0x7fffffu) == 0) continue;
+#pragma unroll 1
+    for (int pass = 0; pass * u.kRowsPass < u.n; ++pass) {
+      uint4 x[2];
+      float c[8], s[8], va[8], vb[8], lo[8], hi[8];
+      u.load(pass, h, x);
+      u.angles(pass, c, s);
+      unpack8<T>(va, x[0]);
+      unpack8<T>(vb, x[1]);
+      to_pairs<IL>(lo, hi, va, vb);
+      const auto code = [&](int k, double l, double h) { lo[k] = to_odd(l / scale), hi[k] = to_odd(h / scale); };
+      if (key) {
+        key_pairs<T>(p, lane, c, s, lo, hi, code);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) code(k, lo[k], hi[k]);
+      }
+      u.store(pass, lo, hi, 1.f, caches + h * p.kv_stride_h + off * p.kv_stride_t);
+    }
+  }
+}
+
+// A CTA's units, f(team, row, seq, place, left, first head, last + 1, key) each: by the CTA's threads or by a warp's.
+template <int N>
+using Team = std::integral_constant<int, N>;
+template <bool ONE, typename F>
+__device__ __forceinline__ void each_units(const RotaryCache &a, F f) {
   const fa_rotary_cache_args &p = a.p;
-  const Lane<LPR, IL> lane(p.rotary_dim);
   const int per_row = 2 * p.num_kv_heads, warp = threadIdx.x / 32, lane_id = threadIdx.x & 31;
   if (ONE) {
     const int64_t i = (int64_t)blockIdx.x * (kCacheThreads / 32) + warp;
     const int row = (int)(i / per_row), rest = (int)(i % per_row);
     if (row >= p.num_tokens) return;
     const Token t = find_token(p, row);
-    if (t.valid)
-      units_of<T, LPR, IL, 32>(p, lane, row, t.seq, t.place, 1, rest / 2, rest / 2 + 1, rest % 2 == 0, nullptr,
-                                   nullptr);
+    if (t.valid) f(Team<32>(), row, t.seq, t.place, 1, rest / 2, rest / 2 + 1, rest % 2 == 0);
     return;
   }
-  __shared__ uint32_t shared_most[2 * kCacheThreads / 32];
-  __shared__ float4 kept[kKept * 4 * kCacheThreads];
   const int tile = blockIdx.x / a.unit_ctas_y, y = blockIdx.x % a.unit_ctas_y;
   const Token t = find_token(p, tile * kTile + lane_id);
   const bool leads = t.valid && (t.first || t.place == 0 || t.place % p.block_size == 0);
@@ -480,18 +527,39 @@ __device__ __forceinline__ void unit_part(const RotaryCache &a) {
   const int per_block = 2 * a.unit_chunks, items = __popc(several) * per_block;
   for (int i = y; i < items; i += a.unit_ctas_y) {
     const int from = __fns(several, 0, i / per_block + 1), rest = i % per_block, h = rest / 2 * a.unit_heads;
-    units_of<T, LPR, IL, kCacheThreads>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from),
-                                        from_lane(t.left, from), h, min(h + a.unit_heads, p.num_kv_heads), rest % 2 == 0,
-                                        shared_most, kept);
-    __syncthreads();   // shared_most is the next one's
+    f(Team<kCacheThreads>(), tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from), from_lane(t.left, from), h,
+      min(h + a.unit_heads, p.num_kv_heads), rest % 2 == 0);
+    __syncthreads();   // the shared memory is the next one's
   }
   // single tokens: a warp for each and head
   const int ones = __popc(single) * per_row;
   for (int i = y * (kCacheThreads / 32) + warp; i < ones; i += a.unit_ctas_y * (kCacheThreads / 32)) {
     const int from = __fns(single, 0, i / per_row + 1), rest = i % per_row;
-    units_of<T, LPR, IL, 32>(p, lane, tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from), 1, rest / 2,
-                             rest / 2 + 1, rest % 2 == 0, nullptr, nullptr);
+    f(Team<32>(), tile * kTile + from, from_lane(t.seq, from), from_lane(t.place, from), 1, rest / 2, rest / 2 + 1,
+      rest % 2 == 0);
   }
+}
+
+// (a function of its own, at the end, where it takes no registers from the units)
+template <typename T, int LPR, bool IL, bool ONE>
+__device__ __noinline__ void divide_part(const RotaryCache &a) {
+  const Lane<LPR, IL> lane(a.p.rotary_dim);
+  each_units<ONE>(a, [&](auto team, int row, int seq, int place, int left, int h_lo, int h_hi, bool key) {
+    divide_units<T, LPR, IL, decltype(team)::value>(a.p, lane, row, seq, place, left, h_lo, h_hi, key);
+  });
+}
+template <typename T, int LPR, bool IL, bool ONE>
+__device__ __forceinline__ void unit_part(const RotaryCache &a) {
+  __shared__ uint32_t shared_most[ONE ? 1 : 2 * kCacheThreads / 32];
+  __shared__ float4 kept[ONE ? 1 : kKept * 4 * kCacheThreads];
+  const Lane<LPR, IL> lane(a.p.rotary_dim);
+  uint32_t mantissas = 0;
+  each_units<ONE>(a, [&](auto team, int row, int seq, int place, int left, int h_lo, int h_hi, bool key) {
+    mantissas |= units_of<T, LPR, IL, decltype(team)::value>(a.p, lane, row, seq, place, left, h_lo, h_hi, key, shared_most, kept);
+  });
+  // (with barriers: a team's threads see the scales that one of them wrote)
+  if (ONE) __syncwarp();
+  if (ONE ? mantissas != 0 : __syncthreads_or(mantissas != 0)) divide_part<T, LPR, IL, ONE>(a);
 }
 
 // UNITS: 0 none (a cache of 16 bits), 1 of one token each, 2 of up to a block's

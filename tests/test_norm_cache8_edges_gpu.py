@@ -109,3 +109,54 @@ def test_starts_that_reach_beyond_the_rows(held):
     b.qkv = b.qkv[:3]
     d = b.device()
     b.check(b.call(d), d)
+
+
+def e4m3_borders():
+    v = cache8.to_e4m3(torch.tensor([m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10) for e in range(16)
+                                     for m in range(8)][:127], dtype=torch.float64))
+    return (v[1:] + v[:-1]) / 2
+
+
+@pytest.mark.parametrize("past,new,starts", [(9, 5, True), (30, 70, True), (3, 1, True), (40, 1, False)])
+@pytest.mark.parametrize("scale", [0.3, 1.7e-3, 1.0, 0.25])
+def test_keys_next_to_a_border_between_codes(scale, past, new, starts):
+    """Keys that 64 bits tell from a border between two codes and 32 bits do not: angles of 24 bits are made so that a key of an
+    8-bit number and an angle is the border times the scale, to half a step of 32 bits, on either side of it.  Scales of any
+    value, as a user's cache may have them, are kept while they suffice."""
+    D, BS, Hk = 64, 128, 2
+    b = Batch([past], [new], 2, Hk, D, BS, torch.bfloat16, True, norm=None, spread=False, seed=new, starts=starts)
+    b.ks[:], b.vs[:] = scale, scale
+    border = e4m3_borders()
+    border = border[(border > 2.0 ** -6) & (border < 250)]
+    gen = torch.Generator().manual_seed(past)
+    _, k, _ = b.parts(b.qkv)
+    k[..., D // 2:] = 0
+    rows = torch.arange(past, past + new)
+    at = border[torch.randint(0, border.numel(), (new, D // 2), generator=gen)]
+    low = torch.randint(128, 256, (new, D // 2), generator=gen).double()
+    want = at * b.ks[0, 0].double()          # (the scale is fp32)
+    low *= torch.exp2(torch.floor(torch.log2(want)) - 7)
+    k[:, :, :D // 2] = low[:, None].to(torch.bfloat16) * torch.tensor([1.0, -1.0])[None, :, None].to(torch.bfloat16)
+    b.cos[rows] = (want / low).float()
+    b.sin[rows] = 0
+    d = b.device()
+    b.check(b.call(d), d)
+
+
+@pytest.mark.parametrize("scale", [49 / 64, 99 / 512, 105.0, 0.5])
+@pytest.mark.parametrize("new", [16, 60])
+def test_values_on_a_border_between_codes(scale, new):
+    """Values that are a border times the scale: the even one of the two codes.  (A product with the scale's reciprocal misses
+    some of them, of scales that are no powers of two.)"""
+    D, BS = 64, 128
+    b = Batch([3], [new], 1, 1, D, BS, torch.float16, True, spread=False, seed=3)
+    b.ks[:], b.vs[:] = 512.0, scale
+    border = e4m3_borders()
+    exact = border * scale
+    exact = exact[(exact.to(torch.float16).double() == exact) & (exact < 448 * scale / 2)]
+    assert exact.numel() > 30
+    _, _, v = b.parts(b.qkv)
+    v[:] = exact[torch.arange(new * D) % exact.numel()].view(new, 1, D).to(torch.float16)
+    v[:, :, ::3] *= -1
+    d = b.device()
+    b.check(b.call(d), d)
