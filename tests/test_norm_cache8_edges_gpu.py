@@ -160,3 +160,30 @@ def test_values_on_a_border_between_codes(scale, new):
     v[:, :, ::3] *= -1
     d = b.device()
     b.check(b.call(d), d)
+
+
+def test_eps_is_taken_in_64_bits():
+    """Normed keys next to borders between codes, by weights of 24 bits, with an eps that 32 bits change by half a step."""
+    D, BS, new = 64, 16, 16
+    eps = 4.0 * (1 + 2.0 ** -24 - 2.0 ** -40)
+    assert abs(float(torch.tensor(eps, dtype=torch.float32)) / eps - 1) > 2.0 ** -25
+    b = Batch([0] * new, [1] * new, 1, 1, D, BS, torch.bfloat16, True, norm="fp32", spread=False, seed=1)
+    border = e4m3_borders()
+    border = border[(border >= 240) & (border < 448)]
+    q, k, v = b.parts(b.qkv)
+    k[:] = k[:1].clone()          # every sequence has one token, the same one at other positions: angles of 0
+    b.cos[:], b.sin[:] = 1.0, 0.0
+    x = k[0, 0].double()
+    r = 1 / torch.sqrt((x * x).mean() + eps)
+    at = border[torch.arange(D) % border.numel()] / 256.0
+    b.wk = (at / (x * r)).float()
+    lens, table, starts = b.lens, b.table, b.starts
+    d = b.device()
+    kc, vc = d["kc"].view(E4M3), d["vc"].view(E4M3)
+    fa.rotary_and_cache(*b.parts(d["qkv"]), kc, vc, d["lens"], d["table"], d["cos"], d["sin"], query_starts=d["starts"],
+                        q_weight=d["wq"], k_weight=d["wk"], eps=eps, key_scales=d["ks"], value_scales=d["vs"])
+    want, ks = b.kc.view(E4M3).double(), b.ks.double()
+    cache8.rotary_and_cache(q, k, v, want, b.vc.view(E4M3).double(), lens, table, b.cos, b.sin, starts, None, b.wq, b.wk, eps,
+                            False, ks, b.vs.double())
+    assert torch.equal(d["ks"].cpu().double(), ks)
+    assert torch.equal(d["kc"].cpu().view(E4M3).double()[table[:, 0].long()], want[table[:, 0].long()])
