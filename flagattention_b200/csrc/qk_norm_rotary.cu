@@ -273,7 +273,9 @@ __global__ void __launch_bounds__(kNormThreads, kBackwardCtas) qk_norm_rotary_bw
             ax = fmaf(tlo[i], t.wlo[i], fmaf(thi[i], t.whi[i], ax));
             glo[i] = hl * t.wlo[i], ghi[i] = hh * t.whi[i];
           }
-          const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, a.eps));
+          ss = group_sum<LPR>(ss);
+          // (places behind the last position are rows of zeros, which with eps = 0 have no r: 0 for those)
+          const float r = t.l < a.L ? rsqrtf(fmaf(ss, inv_d, a.eps)) : 0.f;
           const float k = group_sum<LPR>(ax) * inv_d * r * r * r;   // dx = r a - k x (in this order: r^3 may be below fp32's range)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {

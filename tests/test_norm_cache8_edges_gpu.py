@@ -187,3 +187,21 @@ def test_eps_is_taken_in_64_bits():
                             False, ks, b.vs.double())
     assert torch.equal(d["ks"].cpu().double(), ks)
     assert torch.equal(d["kc"].cpu().view(E4M3).double()[table[:, 0].long()], want[table[:, 0].long()])
+
+
+@pytest.mark.parametrize("B,L,D", [(1, 1, 64), (3, 37, 96), (2, 9, 256)])
+def test_eps_of_zero(B, L, D):
+    """Lengths that leave places of the last strip of positions empty: those have no part in the weights' gradients."""
+    gen = torch.Generator().manual_seed(L)
+    q, g = (torch.randn(B, 3, L, D, generator=gen).to(torch.bfloat16) for _ in range(2))
+    w = 1 + 0.3 * torch.randn(D, generator=gen)
+    cos, sin = fa.rotary_tables(L, D)
+    x, ws = q.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y, _ = fa.qk_norm_rotary(x, x.detach(), ws, w.cuda(), cos.cuda(), sin.cuda(), eps=0.0)
+    dx, dw = torch.autograd.grad(y, (x, ws), g.cuda())
+    want = cache8.norm_rotary(q, w, cos, sin, eps=0.0)
+    size = torch.maximum(*(cache8.norm_rotary(q.abs(), w.abs(), cos.abs(), s, eps=0.0).abs() for s in (sin.abs(), -sin.abs())))
+    dx64, dw64, dx_size, dw_size = cache8.norm_rotary_backward(q, w, g, cos, sin, eps=0.0)
+    for got, want, half, terms, size in ((y, want, 2.0 ** -8, 64, size), (dx, dx64, 2.0 ** -8, 128, dx_size),
+                                         (dw, dw64, 2.0 ** -24, 256, dw_size)):
+        assert ((got.detach().cpu().double() - want).abs() <= half * want.abs() * (1 + half) + terms * U * size).all()
