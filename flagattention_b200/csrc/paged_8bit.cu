@@ -17,7 +17,7 @@
 // The scale of K goes into the score.  The scale of V cannot go into the accumulator, which many blocks share, nor into
 // P alone, whose 16 bits would not hold its range: a token's weight in O is exp2(score) 2^E f for a scale 2^E f, 1 <= f < 2,
 // and O has a running reference of its own over score + E, beside the maximum that the sum of the softmax goes by.  So
-// weights stay in range whatever the scales are (0 too: E = -inf).
+// weights stay in range whatever the scales are.
 // bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): elements down to 2^-38 of
 // the maximum keep their bits or lose less than 2^-40 of it.
 #include <cfloat>
@@ -83,12 +83,12 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src));
 }
-// scale = 2^exponent x fraction, 1 <= fraction < 2; 0 (and what is below the normal numbers) has exponent -inf, an
-// infinity or NaN is its own fraction
+// scale = 2^exponent x fraction, 1 <= fraction < 2; below the normal numbers, 0 among them, exponent -126 and a fraction below
+// 1, whose weights keep fewer bits (off by 2^-31 of 2^-126 at most); an infinity or NaN is its own fraction
 __device__ __forceinline__ void split_scale(float scale, float &exponent, float &fraction) {
   const uint32_t bits = __float_as_uint(scale), e = bits >> 23 & 255u;
-  exponent = e == 255u ? 0.f : e ? (float)((int)e - 127) : -INFINITY;
-  fraction = e == 255u ? scale : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+  exponent = e == 255u ? 0.f : (float)(max((int)e, 1) - 127);
+  fraction = e == 255u ? scale : e ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : scale * 0x1p126f;
 }
 
 // an 8 x 8 matrix of 16-bit numbers, two of row lane / 4 a lane, into its transpose in the same layout
@@ -520,9 +520,11 @@ __global__ void __launch_bounds__(Paged8Cfg<D, NQ>::kWarps * 32, Paged8Cfg<D, NQ
       const float4 v = *reinterpret_cast<const float4 *>(merge + (w2 * C::kRows + row) * KD + c4 * 4);
       o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
     }
-    // from the reference of O to that of the sum; a sequence without tokens has 0, a NaN stays one
-    const float inv = l == 0.f ? 0.f : (ww == -INFINITY ? 1.f : fast_exp2(ww - kLift - mm)) / l;
-    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    // from the reference of O to that of the sum, in two steps where one would be below the normal numbers; a sequence without
+    // tokens has 0, a NaN stays one
+    const float by = ww - kLift - mm, rest = by < -100.f ? 0x1p-64f : 1.f;
+    const float inv = l == 0.f ? 0.f : (ww == -INFINITY ? 1.f : fast_exp2(by < -100.f ? by + 64.f : by)) / l;
+    o.x = o.x * inv * rest, o.y = o.y * inv * rest, o.z = o.z * inv * rest, o.w = o.w * inv * rest;
     const int qh = qh0 + row;
     if (a.partition_size > 0) {
       const int P = (a.max_context_len + a.partition_size - 1) / a.partition_size;

@@ -205,3 +205,35 @@ def test_eps_of_zero(B, L, D):
     for got, want, half, terms, size in ((y, want, 2.0 ** -8, 64, size), (dx, dx64, 2.0 ** -8, 128, dx_size),
                                          (dw, dw64, 2.0 ** -24, 256, dw_size)):
         assert ((got.detach().cpu().double() - want).abs() <= half * want.abs() * (1 + half) + terms * U * size).all()
+
+
+@pytest.mark.parametrize("exponent", [-112, -118, -126, -127, -131])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("group", [2, 16])
+def test_the_smallest_scales_of_values(exponent, splits, group):
+    """bf16 holds 2^-126, and less in fewer bits, so scales down to there and below (codes are up to 448) are seen in the output.
+
+    The bound of test_paged_8bit_gpu.py, and half of bf16's least step; fp32's own, 2^-149, once for each partition."""
+    from test_paged_8bit_gpu import made
+    x = made([700, 33, 16], 2 * group, 2, 128, 16, torch.bfloat16, seed=group)
+    q, kc, vc, ks, vs, lens, bt = x
+    last = vs[-1].clone()
+    vs[:] = 2.0 ** exponent
+    vs[1::3] = 1.25 * 2.0 ** (exponent + 1)
+    vs[-1] = last
+    out = fa.paged_attention_8bit(*(t.cuda() for t in x), 128 ** -0.5, 700, splits)
+    want, size, most = cache8.paged_attention_8bit(*x, 128 ** -0.5)
+    assert want.abs().max() > 2.0 ** exponent
+    half = 2.0 ** -8
+    bound = half * want.abs() * (1 + half) + (64 * 2.0 ** -23 * most + 2.0 ** -20 + 2.0 ** -17) * size + 2.0 ** -134 + 2.0 ** -147
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+
+
+def test_small_scales_beside_large_ones_and_of_keys():
+    """A scale below the normal numbers is a positive number like others: of a key, and of a value beside a larger one."""
+    from test_paged_8bit_gpu import check, made
+    x = made([200, 48], 8, 2, 64, 16, torch.float16, seed=4)
+    q, kc, vc, ks, vs, lens, bt = x
+    ks[:-1:2] = 2.0 ** -133
+    vs[1:-1:3] = 2.0 ** -140
+    check(fa.paged_attention_8bit(*(t.cuda() for t in x), 0.125, 200), x, 0.125)
