@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::kWarps * 32) paged_decode_kernel(
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
     const int qh = qh0 + row;
     if (a.partition_size > 0) {
-      const int P = (a.max_context_len + a.partition_size - 1) / a.partition_size;
+      const int P = partitions_of(a);
       const int64_t pi = ((int64_t)seq * a.num_q_heads + qh) * P + part;
       *reinterpret_cast<float4 *>(a.part_out + pi * D + c4 * 4) = o;
       if (c4 == 0) {
@@ -368,10 +368,10 @@ __global__ void __launch_bounds__(kReduceThreads) paged_reduce_kernel(const fa_p
   const int seq = blockIdx.x, qh = blockIdx.y;
   const int D = a.head_size, cols = D / 4, groups = blockDim.x / cols;
   const int g = threadIdx.x / cols, c4 = threadIdx.x % cols;
-  const int P = (a.max_context_len + a.partition_size - 1) / a.partition_size;
+  const int P = partitions_of(a);
   const int ctx = context_len(a, seq);
   const int size = partition_tokens(a, z, lane_lens(a, z), ctx, P);
-  const int np = min(P, (ctx + size - 1) / size);
+  const int np = ctx > 0 ? min(P, (ctx - 1) / size + 1) : 0;
   // launched beside the decode kernel's last CTAs (reduce()): its results are there from here on
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int64_t base = ((int64_t)seq * a.num_q_heads + qh) * P;
@@ -454,9 +454,7 @@ static int launch_paged(const fa_paged_args *a, const Sizing &z, cudaStream_t st
   if (int st = ensure_dyn_smem(kern, C::kTotal, &attr_done)) return st;
   const int G = a->num_q_heads / a->num_kv_heads;
   const int q_tiles = (G + 15) / 16;
-  const int P = a->partition_size > 0
-                    ? (a->max_context_len + a->partition_size - 1) / a->partition_size
-                    : 1;
+  const int P = a->partition_size > 0 ? partitions_of(*a) : 1;
   dim3 grid(a->num_seqs, a->num_kv_heads * q_tiles, P);
   kern<<<grid, C::kWarps * 32, C::kTotal, stream>>>(*a, z);
   FA_CHECK_LAUNCH();
@@ -532,8 +530,8 @@ extern "C" int fa_paged_attention(const fa_paged_args *a, int32_t finest, int32_
 }
 
 extern "C" int64_t fa_paged_workspace_bytes(const fa_paged_args *a) {
-  if (!a || a->partition_size <= 0) return 0;
-  const int64_t P = (a->max_context_len + a->partition_size - 1) / a->partition_size;
+  if (!a || a->partition_size <= 0 || a->max_context_len <= 0) return 0;
+  const int64_t P = partitions_of(*a);
   const int64_t rows = (int64_t)a->num_seqs * a->num_q_heads * P;
   return rows * a->head_size * 4 + 2 * rows * 4;
 }
@@ -608,7 +606,7 @@ extern "C" int fa_paged_attention_noalloc(const fa_paged_args *a, void *stream) 
   unsigned char *base = nullptr;
   st = paged_scratch_base(&base);
   if (st != FA_OK) return st;
-  const int64_t P = (local.max_context_len + local.partition_size - 1) / local.partition_size;
+  const int64_t P = partitions_of(local);
   const int64_t rows = (int64_t)local.num_seqs * local.num_q_heads * P;
   // layout inside the array: partial outputs, then running maxima, then running sums.  Nothing
   // has to be zeroed: the decode kernel writes every (row, partition) slot the reducer later reads.

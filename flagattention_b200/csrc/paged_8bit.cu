@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(Paged8Cfg<D, NQ>::kWarps * 32, Paged8Cfg<D, NQ
     o.x = o.x * inv * rest, o.y = o.y * inv * rest, o.z = o.z * inv * rest, o.w = o.w * inv * rest;
     const int qh = qh0 + row;
     if (a.partition_size > 0) {
-      const int P = (a.max_context_len + a.partition_size - 1) / a.partition_size;
+      const int P = partitions_of(a);
       const int64_t pi = ((int64_t)seq * a.num_q_heads + qh) * P + part;
       *reinterpret_cast<float4 *>(a.part_out + pi * D + c4 * 4) = o;
       if (c4 == 0) {
@@ -584,7 +584,7 @@ static int launch_8bit(const fa_paged_8bit_args *p, const Sizing &z, cudaStream_
   static unsigned long long attr_done = 0;  // per instantiation, one bit per device
   if (int st = ensure_dyn_smem(kern, C::kTotal, &attr_done)) return st;
   const int q_tiles = (a->num_q_heads / a->num_kv_heads + 15) / 16;
-  const int P = a->partition_size > 0 ? (a->max_context_len + a->partition_size - 1) / a->partition_size : 1;
+  const int P = a->partition_size > 0 ? partitions_of(*a) : 1;
   kern<<<dim3(a->num_seqs * a->num_kv_heads * q_tiles, P), C::kWarps * 32, C::kTotal, stream>>>(*p, z);
   FA_CHECK_LAUNCH();
   return FA_OK;

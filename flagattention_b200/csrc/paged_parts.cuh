@@ -22,6 +22,9 @@ __device__ __forceinline__ int context_len(const fa_paged_args &a, int seq) {
   return a.context_lens ? a.context_lens[seq] : a.max_context_len;
 }
 
+// the partitions of a row in the workspace (the bound and a partition may come to more than 32 bits)
+__host__ __device__ inline int partitions_of(const fa_paged_args &a) { return (a.max_context_len - 1) / a.partition_size + 1; }
+
 // How the kernels size the partitions of fa_paged_attention from the lengths themselves; finest == 0: every sequence
 // takes a.partition_size.  Sizes are finest * 2^k.
 struct Sizing {

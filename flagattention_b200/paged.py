@@ -85,7 +85,7 @@ def size_partitions(base, num_seqs, ctas, max_context_len, num_sms, fill=0.8, ma
         # few long contexts: one wave of equal partitions, `slots` CTAs an SM (131071 tokens, 8 kv heads, codes of 8 bits, an
         # earlier kernel: 59 us so, 76 with the power of two below, 71 with the one above)
         parts = slots * num_sms // pairs
-        finest = size = max(base, _cdiv(_cdiv(max_context_len, parts), 128) * 128)
+        finest = size = min(max(base, _cdiv(_cdiv(max_context_len, parts), 128) * 128), 1 << 24)   # (what the library takes)
         while finest % 32 == 0 and finest >= 256:   # for contexts far below the bound
             finest //= 2
         return (0, base, base, 0, 1) if max_context_len <= size else (size, finest, size, 0, parts)
@@ -96,6 +96,9 @@ def size_partitions(base, num_seqs, ctas, max_context_len, num_sms, fill=0.8, ma
     while size < coarsest and (ctas * _cdiv(max_context_len, 2 * size) >= fill * num_sms
                                or num_seqs * ctas * _cdiv(max_context_len, size) > many * num_sms):
         size *= 2
+    while slots and _cdiv(max_context_len, size) > 4096:   # bounds that are none: of the workspace, and of the grid (65535)
+        size *= 2
+    coarsest = max(coarsest, size)
     if max_context_len <= size:
         return 0, base, coarsest, 0, 1
     pairs = num_seqs * ctas
@@ -333,7 +336,7 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
     _check_caches(key_cache, value_cache, num_kv_heads, head_size, 16)
     _check_scales(key_cache, key_scales, value_scales)
     max_context_len = int(max_context_len)
-    assert max_context_len > 0 and num_splits >= 0
+    assert 0 < max_context_len < 2 ** 31 and num_splits >= 0
     context_lens = _int32(context_lens, "context_lens", num_seqs, query.device)
     block_tables = _table_ready(block_tables, num_seqs, query.device)
     query = _rows_ready(query)
