@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(kNormThreads, kBackwardCtas) qk_norm_rotary_bw
         t.b = (int)(rest % a.B);
         t.turn_to(a, (int)(rest / a.B) * kRows + group);
         const int h0 = chunk * a.per_cta[e], count = min(side.heads - h0, a.per_cta[e]);
+        // (places behind the last position are rows of zeros, which would have no r with eps = 0)
+        const float eps = t.l < a.L ? a.eps : 1.f;
         const bool here = t.live && t.l < a.L;
         T *y = static_cast<T *>(side.y) + t.b * side.sy.b + (here ? t.l * side.sy.l : 0) + h0 * side.sy.h;
 #pragma unroll 1
@@ -273,9 +275,7 @@ __global__ void __launch_bounds__(kNormThreads, kBackwardCtas) qk_norm_rotary_bw
             ax = fmaf(tlo[i], t.wlo[i], fmaf(thi[i], t.whi[i], ax));
             glo[i] = hl * t.wlo[i], ghi[i] = hh * t.whi[i];
           }
-          ss = group_sum<LPR>(ss);
-          // (places behind the last position are rows of zeros, which with eps = 0 have no r: 0 for those)
-          const float r = t.l < a.L ? rsqrtf(fmaf(ss, inv_d, a.eps)) : 0.f;
+          const float r = rsqrtf(fmaf(group_sum<LPR>(ss), inv_d, eps));
           const float k = group_sum<LPR>(ax) * inv_d * r * r * r;   // dx = r a - k x (in this order: r^3 may be below fp32's range)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
