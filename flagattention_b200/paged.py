@@ -317,7 +317,9 @@ def attention_8bit(query, key_cache, value_cache, key_scales, value_scales, cont
     query [num_seqs, kv_heads * group, head] fp16 / bf16, head 16, 32, 64, 128 or 256; block a multiple of 16;
     context_lens [num_seqs] and block_tables [num_seqs, max_blocks] as in `attention`.  A sequence of length 0 gives 0;
     one whose table names a block that the cache does not have gives NaN.  fp32 sums and statistics, the output rounded
-    once.  `rotary_and_cache` writes such caches."""
+    once.  `rotary_and_cache` writes such caches.  Not differentiable: operands that require gradients give an output that
+    does not.  Several rows of one sequence (a chunk of a prompt) are given as sequences of their own, each with its place + 1
+    as its length and its sequence's row of the table; each reads the cache once."""
     if type(max_context_len) is int and max_context_len > 0 and num_splits == 0 and _native.usable(query):
         out = _native_8bit(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
                            max_context_len)
@@ -398,7 +400,8 @@ def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, bl
 
     Rows behind the last sequence, or in front of theirs (context_lens smaller than its rows; 0 for an idle slot of a
     padded batch), are written nowhere and come back as 0.  A block that is written to must belong to one sequence only:
-    otherwise what its places hold afterwards is not defined."""
+    otherwise what its places hold afterwards is not defined.  Not differentiable: operands that require gradients give an
+    output that does not."""
     if _native.usable(query):
         out = _native.load().rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, block_tables, cos,
                                               sin, query_starts, positions, q_weight, k_weight, key_scales, value_scales,

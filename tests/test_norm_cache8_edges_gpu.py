@@ -237,3 +237,44 @@ def test_small_scales_beside_large_ones_and_of_keys():
     ks[:-1:2] = 2.0 ** -133
     vs[1:-1:3] = 2.0 ** -140
     check(fa.paged_attention_8bit(*(t.cuda() for t in x), 0.125, 200), x, 0.125)
+
+
+@pytest.mark.parametrize("held", [True, False])
+def test_chunks_behind_cached_tokens_attend_row_by_row(held):
+    """Rows of prompts as sequences of their own, a length and a row of the table each, over what rotary_and_cache wrote.
+
+    The bound of test_paged_8bit_gpu.py, and what the least numbers of fp16 cost, which the old codes here (any bits) show: a
+    weight exp2(score - reference) s, s the scale (1 for 16 bits), goes in as an fp16 value, cut, and an fp16 remainder that
+    is kept at 2^-24 or more (split_weights): off by 2^-24 where it is small, whatever the value beside it.  References are
+    at most the largest score (and scale), 8-bit weights stand 2^6 above theirs: 2^-30 (16 bits: 2^-24) max(p s) sum |code|
+    of the output, p the softmax."""
+    b = Batch([20, 0, 33], [13, 40, 1], 8, 2, 64, 16, torch.float16, held, seed=5, spread=False)
+    d = b.device()
+    q = b.call(d)
+    starts, lens = d["starts"].long(), d["lens"].long()
+    rows = torch.arange(q.shape[0], device="cuda")
+    seq = torch.searchsorted(starts, rows, right=True) - 1
+    row_lens = (lens[seq] - (starts[seq + 1] - 1 - rows)).to(torch.int32)
+    table = d["table"][seq]
+    assert row_lens.tolist() == list(range(21, 34)) + list(range(1, 41)) + [34]
+    kc, vc, ks, vs = (d[n] for n in ("kc", "vc", "ks", "vs"))
+    if held:
+        kc, vc = kc.view(E4M3), vc.view(E4M3)
+        o = fa.paged_attention_8bit(q, kc, vc, ks, vs, row_lens, table, 0.125, 40)
+    else:
+        ks = vs = torch.ones(kc.shape[:2], device="cuda")
+        o = fa.paged_attention(q, kc, vc, row_lens, table, 0.125, 40)
+    x = [t.cpu() for t in (q, kc, vc, ks, vs, row_lens, table)]
+    want, size, most = cache8.paged_attention_8bit(*x, 0.125)
+    q, kc, vc, ks, vs = (t.double() for t in x[:5])
+    least = torch.zeros_like(want)
+    for i, n in enumerate(row_lens.tolist()):
+        ids = x[6][i].long()
+        k, v = (c[ids].transpose(0, 1).flatten(1, 2)[:, :n] for c in (kc * ks[..., None, None], vc))
+        s = vs[ids].t().repeat_interleave(16, 1)[:, :n]
+        p = torch.softmax(q[i].view(2, 4, 64) @ k.transpose(1, 2) * 0.125, -1)
+        top = (p * s[:, None]).amax(-1, keepdim=True)
+        least[i] = (2.0 ** (-30 if held else -24) * top * v.abs().sum(1, keepdim=True)).flatten(0, 1)
+    half = 2.0 ** -11
+    bound = half * want.abs() * (1 + half) + (64 * 2.0 ** -23 * most + 2.0 ** -20 + 2.0 ** -17) * size + least + 2.0 ** -25
+    assert o.isfinite().all() and ((o.cpu().double() - want).abs() <= bound).all()
