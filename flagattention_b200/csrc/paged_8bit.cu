@@ -18,8 +18,8 @@
 // P alone, whose 16 bits would not hold its range: a token's weight in O is exp2(score) 2^E f for a scale 2^E f, 1 <= f < 2,
 // and O has a running reference of its own over score + E, beside the maximum that the sum of the softmax goes by.  So
 // weights stay in range whatever the scales are.
-// bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): elements down to 2^-38 of
-// the maximum keep their bits or lose less than 2^-40 of it.
+// bf16 queries are brought to fp16 by a power of two for each row, its maximum to [2^14, 2^15): an element keeps
+// its bits or loses 2^-39 of the maximum at most (half of fp16's least step).
 #include <cfloat>
 #include <climits>
 
@@ -36,7 +36,8 @@ template <int D, int NQ>
 struct Paged8Cfg {
   static constexpr int kD = D < 64 ? 64 : D;   // shorter heads are padded with zeros in shared memory
   static constexpr int kWarps = 4, kRows = 8 * NQ;
-  // Warps as the registers allow without spills, groups as short as the bookkeeping between them allows.  us for 64
+  // Warps as the registers allow (two columns at head 64 and below spill 20 to 32 bytes), groups as short as the bookkeeping between
+  // them allows.  us for 64
   // sequences, tokens of a group x CTAs: head 128, 8 kv heads of 4, 1K-32K tokens 16 x 4 355, 32 x 3 355 (one sequence of
   // 131071: 51, 52), 32 x 2 362, 2 kv heads of 16, 1K-16K 16 x 4 94, 16 x 3 with queries in registers 102, 32 x 3 106; head
   // 64, 8 kv heads of 4, 1K-16K 32 x 4 115, 16 x 4 124, 16 x 5 118, 64 x 3 121; head 256, 32 sequences of 4 kv heads 16 x 2

@@ -562,7 +562,7 @@ __device__ __forceinline__ void unit_part(const RotaryCache &a) {
   if (ONE ? mantissas != 0 : __syncthreads_or(mantissas != 0)) divide_part<T, LPR, IL, ONE>(a);
 }
 
-// UNITS: 0 none (a cache of 16 bits), 1 of one token each, 2 of up to a block's
+// UNITS: 0 none (a cache of 16 bits), 1 of one token each, 2 of up to a block's (which spill 32 to 68 bytes at 96 registers)
 template <typename T, int LPR, bool IL, int UNITS>
 __global__ void __launch_bounds__(kCacheThreads, UNITS == 1 ? 4 : 5) rotary_cache_kernel(const __grid_constant__ RotaryCache a) {
   if (UNITS && (int)blockIdx.x < a.unit_ctas) unit_part<T, LPR, IL, UNITS == 1>(a);
