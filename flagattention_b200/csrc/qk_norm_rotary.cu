@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kNormThreads, kForwardCtas) qk_norm_rotary_fwd
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     ll[i] = t.c[i] * t.wlo[i], hh[i] = t.c[i] * t.whi[i];
-    lh[i] = t.s[i] * t.whi[i], hl[i] = t.s[i] * t.wlo[i];
+    lh[i] = t.turns ? t.s[i] * t.whi[i] : 0.f, hl[i] = t.turns ? t.s[i] * t.wlo[i] : 0.f;
   }
   x += t.h_lo * side.sx.h;
   y += t.h_lo * side.sy.h;

@@ -210,7 +210,7 @@ __device__ __forceinline__ void row_part(const RotaryCache &a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float c = ll[i], s = lh[i], l = norm ? wlo[i] : 1.f, h = norm ? whi[i] : 1.f;
-      ll[i] = c * l, hh[i] = c * h, lh[i] = s * h, hl[i] = s * l;
+      ll[i] = c * l, hh[i] = c * h, lh[i] = lane.turns ? s * h : 0.f, hl[i] = lane.turns ? s * l : 0.f;
     }
   }
   const float inv_d = 1.f / p.head_size;

@@ -278,3 +278,27 @@ def test_chunks_behind_cached_tokens_attend_row_by_row(held):
     half = 2.0 ** -11
     bound = half * want.abs() * (1 + half) + (64 * 2.0 ** -23 * most + 2.0 ** -20 + 2.0 ** -17) * size + least + 2.0 ** -25
     assert o.isfinite().all() and ((o.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_weight_that_is_no_number_stays_in_its_column(interleaved):
+    """Behind the rotated elements: one column of the queries and the keys, whatever the cache."""
+    D, R = 128, 64
+    for held in (True, False):
+        b = Batch([3, 20], [18, 5], 2, 2, D, 16, torch.bfloat16, held, R=R, seed=1, interleaved=interleaved)
+        b.wq[R + 3], b.wk[R + 9], b.wk[D - 1] = float("nan"), float("inf"), float("nan")
+        d = b.device()
+        out = b.call(d)
+        want_q, kc, vc, ks, vs = b.expected()
+        assert not same_where_not_finite(out, want_q)[:, :, R + 3].any()
+        if held:
+            got = d["kc"].cpu().view(E4M3).double()
+            assert ((got == kc) | (got.isnan() & kc.isnan())).all() and torch.equal(d["ks"].cpu().double(), ks)
+        else:
+            same_where_not_finite(d["kc"], kc)
+    q, w = torch.randn(1, 2, 9, D, device="cuda").half(), torch.ones(D, device="cuda")
+    w[R + 3] = float("nan")
+    y, _ = fa.qk_norm_rotary(q, q, w, w, *fa.rotary_tables(9, R, device="cuda"), interleaved=interleaved)
+    bad = torch.zeros(D, dtype=torch.bool, device="cuda")
+    bad[R + 3] = True
+    assert torch.equal(y.isnan(), bad.expand_as(y))
