@@ -80,7 +80,7 @@ class RotaryCacheArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "dtype", "num_tokens", "num_seqs", "num_q_heads", "num_kv_heads", "head_size", "rotary_dim", "interleaved",
         "block_size", "num_blocks", "table_cols", "block_table_is_i64", "table_rows", "weight_is_f32")] + \
-        [("eps", ctypes.c_double)] + \
+        [("eps", ctypes.c_float), ("eps_low", ctypes.c_float)] + \
         [f for n in ("query", "key", "value", "out")
          for f in ((n, ctypes.c_void_p), (n[0] + "_stride_t", ctypes.c_int64), (n[0] + "_stride_h", ctypes.c_int64))] + \
         [("key_cache", ctypes.c_void_p), ("value_cache", ctypes.c_void_p), ("kv_stride_b", ctypes.c_int64),
@@ -175,7 +175,7 @@ _SHAPE = struct.Struct("@8i2f2Q")                                   # FlashShape
 _TENSOR4 = struct.Struct("@P3q")                                    # Tensor4
 PAGED_ARGS = struct.Struct("@9ifP2q2P3q2PqP2q3Pi4x")                # PagedArgs
 NORM_ROTARY_ARGS = struct.Struct("@10if5Pq")                        # NormRotaryArgs
-ROTARY_CACHE_ARGS = struct.Struct("@14id" + "P2q" * 4 + "2P3q5Pq5P")   # RotaryCacheArgs
+ROTARY_CACHE_ARGS = struct.Struct("@14i2f" + "P2q" * 4 + "2P3q5Pq5P")   # RotaryCacheArgs
 PAGED_8BIT_ARGS = struct.Struct(PAGED_ARGS.format + "2P2i")         # Paged8bitArgs
 _SIGNATURES = {
     "fa_flash_keep_bits_bytes": "p", "fa_flash_fwd_keep": "pppppp" + "plp", "fa_flash_bwd_keep": "p" * 11 + "lplp",

@@ -723,7 +723,7 @@ Tensor rotary_and_cache(const Tensor *const (&t)[9], const Tensor (&o)[6], doubl
   a.interleaved = interleaved, a.block_size = (int32_t)kc.size(2), a.num_blocks = (int32_t)kc.size(0);
   a.table_cols = (int32_t)table.size(1), a.block_table_is_i64 = table.scalar_type() == at::kLong;
   a.table_rows = (int32_t)cos.size(0), a.weight_is_f32 = qw.defined() && qw.scalar_type() == at::kFloat;
-  a.eps = eps;
+  a.eps = (float)eps, a.eps_low = std::isfinite(a.eps) ? (float)(eps - (double)a.eps) : 0.f;
   a.query = q.data_ptr(), a.q_stride_t = stride(q, 0), a.q_stride_h = stride(q, 1);
   a.key = k.data_ptr(), a.k_stride_t = stride(k, 0), a.k_stride_h = stride(k, 1);
   a.value = v.data_ptr(), a.v_stride_t = stride(v, 0), a.v_stride_h = stride(v, 1);

@@ -226,7 +226,7 @@ __device__ __forceinline__ void row_part(const RotaryCache &a) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(va[i], va[i], fmaf(vb[i], vb[i], ss));
-        r = rsqrtf(fmaf(lanes_sum<LPR>(ss), inv_d, (float)p.eps));
+        r = rsqrtf(fmaf(lanes_sum<LPR>(ss), inv_d, p.eps));
       }
       to_pairs<IL>(lo, hi, va, vb);
 #pragma unroll
@@ -280,7 +280,7 @@ __device__ __forceinline__ void key_pairs(const fa_rotary_cache_args &p, const L
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) ss += (double)lo[k] * lo[k] + (double)hi[k] * hi[k];
-    r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + p.eps);
+    r = 1.0 / sqrt(lanes_sum<LPR>(ss) / p.head_size + ((double)p.eps + p.eps_low));
     lane.template weights<T>(p, p.k_weight, wlo, whi);
   }
   if (lane.turns) {

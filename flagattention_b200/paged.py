@@ -4,7 +4,9 @@ Mirrors src/flag_attn/paged.py:6-163: same arguments, same split rule
 (num_splits == 0 picks it automatically, 1 disables it, > 1 fixes the count),
 returns a new tensor shaped like `query`.
 """
+import ctypes
 import functools
+import math
 
 import torch
 
@@ -295,6 +297,12 @@ def _rows_ready(t):
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def _two_parts(x):
+    """A number as fp32 and what that leaves out, fp32 as well."""
+    high = ctypes.c_float(x).value
+    return high, float(x) - high if math.isfinite(high) else 0.0
+
+
 def _stride(t, i):
     return t.stride(i) if t.shape[i] > 1 else 0
 
@@ -453,7 +461,7 @@ def rotary_and_cache(query, key, value, key_cache, value_cache, context_lens, bl
     args = _C.ROTARY_CACHE_ARGS.pack(
         dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size, 2 * cos.shape[1], 1 if interleaved else 0,
         key_cache.shape[2], key_cache.shape[0], block_tables.shape[1], 1 if block_tables.dtype == torch.int64 else 0,
-        cos.shape[0], 1 if q_weight is not None and q_weight.dtype == torch.float32 else 0, eps,
+        cos.shape[0], 1 if q_weight is not None and q_weight.dtype == torch.float32 else 0, *_two_parts(eps),
         *(x for t in (query, key, value, out) for x in (t.data_ptr(), _stride(t, 0), _stride(t, 1))),
         key_cache.data_ptr(), value_cache.data_ptr(), kb, kh, kt, ptr(key_scales), ptr(value_scales),
         context_lens.data_ptr(), ptr(query_starts), block_tables.data_ptr(), block_tables.stride(0), ptr(positions),

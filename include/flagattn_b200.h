@@ -450,7 +450,7 @@ int fa_qk_norm_rotary_bwd(const fa_norm_rotary_args *a, const fa_tensor4 *q, con
 typedef struct fa_rotary_cache_args {
   int32_t dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size, rotary_dim, interleaved;
   int32_t block_size, num_blocks, table_cols, block_table_is_i64, table_rows, weight_is_f32;
-  double eps;   /* (codes of 8 bits go by 64-bit arithmetic) */
+  float eps, eps_low;   /* eps_low: what eps has beyond 32 bits, 0 for nothing (codes of 8 bits go by 64-bit arithmetic) */
   const void *query;
   int64_t q_stride_t, q_stride_h;
   const void *key;

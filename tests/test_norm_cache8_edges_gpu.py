@@ -162,8 +162,12 @@ def test_values_on_a_border_between_codes(scale, new):
     b.check(b.call(d), d)
 
 
-def test_eps_is_taken_in_64_bits():
+@pytest.mark.parametrize("native", [True, False])
+def test_eps_is_taken_in_64_bits(native, monkeypatch):
     """Normed keys next to borders between codes, by weights of 24 bits, with an eps that 32 bits change by half a step."""
+    if not native:
+        from flagattention_b200 import _native
+        monkeypatch.setattr(_native, "usable", lambda x: False)
     D, BS, new = 64, 16, 16
     eps = 4.0 * (1 + 2.0 ** -24 - 2.0 ** -40)
     assert abs(float(torch.tensor(eps, dtype=torch.float32)) / eps - 1) > 2.0 ** -25
